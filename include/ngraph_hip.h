@@ -71,6 +71,8 @@ extern "C" {
 #define NGH_I16     5          /* int16 (plain integers, no scale)          */
 #define NGH_I8      6          /* int8                                      */
 #define NGH_U8      7          /* uint8 (image bytes on the loader side)    */
+#define NGH_BF16    8          /* bfloat16: the operators over rows and parameters further down
+                                  (embedding, block norm, AdamW); fused specs refuse it          */
 
 /* ---- spec flags ---------------------------------------------------------
  * NGH_SPEC_PROBE: run the program but store NOTHING; instead every FLEX16
@@ -474,6 +476,155 @@ int  ngh_graph_end(ngh_context* ctx, ngh_graph** out);
 int  ngh_graph_launch(ngh_context* ctx, ngh_graph* graph);
 int  ngh_graph_nodes(const ngh_graph* graph, int32_t* out_nodes);
 int  ngh_graph_free(ngh_context* ctx, ngh_graph* graph);
+
+/* ---- operators over rows and parameters -----------------------------------------------------
+ * The parts of a language model's training step that are not matrix products.  The reference has
+ * the lookup table and its gradient (op_graph/lookuptable.py:55-115, gpu/lut.py) and composes
+ * norms and optimisers of elementwise kernels (frontends/neon/layer.py:1242-1257,
+ * optimizer.py:446-470); the fused forms here have no counterpart in it.
+ *
+ * Common rules.  Each call launches on the context's stream, on the context's device whatever
+ * device the thread has current, waits for nothing, allocates nothing and keeps nothing: what it
+ * needs between its launches is a workspace of the caller, which may be shared by calls that run
+ * one after the other on one context and must not be by calls that may overlap.  All of them may
+ * be recorded between ngh_graph_begin and ngh_graph_end.  Storage types are NGH_F32, NGH_F16 and
+ * NGH_BF16; arithmetic is fp32 and a result is rounded once, to nearest even.  Strides are in
+ * elements between rows; the elements of a row are consecutive.  Any alignment to the element
+ * is taken; rows that start on 16-byte boundaries and are whole 16-byte pieces run fastest.
+ * Outputs overlap nothing else the call touches, except where an entry says so.  Specs start with
+ * abi_version = NGH_ABI_VERSION; fields that do not apply are zero.                            */
+
+/* Embedding: y[n, :] = scale * table[tokens[n], :], n < rows.  A token equal to pad_idx or outside
+ * [0, vocab) (-1, say, for a place that holds none) gives a row of zeros; pad_idx -1 pads none.  */
+typedef struct ngh_embedding_spec {
+    int32_t  abi_version;
+    int32_t  table_dtype, y_dtype;   /* the same, or an NGH_F32 table and 16-bit rows; gradient: the
+                                        same, or 16-bit rows and an NGH_F32 table                */
+    int32_t  pad_idx;
+    int64_t  rows, vocab, width;     /* rows, vocab < 2^31; width < 2^31                         */
+    const int32_t* tokens;           /* [rows], device                                           */
+    void*    table;                  /* [vocab, width], device; the gradient of the table for
+                                        ngh_embedding_grad                                       */
+    int64_t  table_stride;
+    void*    y;                      /* [rows, width], device; its gradient (only read) for
+                                        ngh_embedding_grad                                       */
+    int64_t  y_stride;
+    float    scale;
+    int32_t  accumulate;             /* gradient only: 0 = every row of the table is written, rows
+                                        whose token does not occur with zeros; 1 = the sums are added
+                                        to the rows whose token occurs, the others are not touched */
+    void*    workspace;              /* gradient only; device, 16-byte aligned                   */
+    size_t   workspace_bytes;
+} ngh_embedding_spec;
+int  ngh_validate_embedding(const ngh_embedding_spec* spec, int32_t gradient);   /* no device needed */
+int  ngh_embedding(ngh_context* ctx, const ngh_embedding_spec* spec);
+/* table[v, :] (+)= scale * sum of y[n, :] over the n with tokens[n] == v.  The tokens are sorted (by
+ * token, then by place) and the rows of a token are added in that order in fp32, split at fixed
+ * places of the sorted list: no atomics on values, the same bits from run to run.              */
+int  ngh_embedding_grad(ngh_context* ctx, const ngh_embedding_spec* spec);
+int  ngh_embedding_grad_workspace(const ngh_embedding_spec* spec, size_t* out_bytes);
+
+/* The norms before and after a block with its gate and residual, in one pass over the rows.  With
+ * N the chosen norm of a row (NGH_NORM_RMS: x / sqrt(mean(x^2) + eps); NGH_NORM_LAYER:
+ * (x - mean(x)) / sqrt(var(x) + eps)):
+ *     u = N(b) * post_gain + post_bias      b, the block's output; without post_norm u = b
+ *     h = residual_scale * x + gate * u     the residual stream after the block
+ *     y = N(h) * gain + bias                what the next block reads
+ * b NULL: there is no block before, h = residual_scale * x.  y NULL: no norm follows.  h NULL: the
+ * stream is not wanted (a first norm whose input is the stream already).  Gains, biases and the
+ * gate may each be NULL (1, 0, 1).  The gate has one row for every gate_rows consecutive rows: 1 a
+ * gate for each row, the rows of a sequence one for each sequence, rows one for all.
+ * y is computed from h before h is rounded.  h may be x itself (the same address and stride).    */
+#define NGH_NORM_RMS   0
+#define NGH_NORM_LAYER 1
+#define NGH_BLOCK_NORM_MAX_WIDTH 16384
+typedef struct ngh_block_norm_spec {
+    int32_t  abi_version;
+    int32_t  kind;                   /* NGH_NORM_*                                               */
+    int32_t  dtype;                  /* x, b, h, y and their gradients                           */
+    int32_t  param_dtype;            /* gains, biases, gate and their gradients: dtype or NGH_F32 */
+    int32_t  post_norm;
+    float    eps, residual_scale;
+    int32_t  reserved;
+    int64_t  rows, width;            /* rows < 2^31; width 1 .. NGH_BLOCK_NORM_MAX_WIDTH         */
+    int64_t  gate_rows;              /* 0 without a gate, else a divisor of rows                 */
+    const void *x, *b;
+    int64_t  x_stride, b_stride;
+    const void *gain, *bias, *post_gain, *post_bias;      /* [width]                              */
+    const void *gate;                /* [rows / gate_rows, width]                                */
+    int64_t  gate_stride;
+    void     *h, *y;                 /* h is only read by ngh_block_norm_grad                    */
+    int64_t  h_stride, y_stride;
+    /* ngh_block_norm_grad only.  In: the gradients of y and of h (dh NULL: none arrives; dy NULL:
+     * no norm follows), h and b.  Out: the gradients of x and b and those of the vectors that are
+     * wanted (NULL: not).  dx may be dh itself, or NULL.                                        */
+    const void *dy, *dh;
+    int64_t  dy_stride, dh_stride;
+    void     *dx, *db;
+    int64_t  dx_stride, db_stride;
+    void     *dgain, *dbias, *dpost_gain, *dpost_bias;    /* [width]                              */
+    void     *dgate;                 /* [rows / gate_rows, width]                                */
+    int64_t  dgate_stride;
+    void*    workspace;              /* device, 16-byte aligned                                  */
+    size_t   workspace_bytes;
+} ngh_block_norm_spec;
+int  ngh_validate_block_norm(const ngh_block_norm_spec* spec, int32_t gradient); /* no device needed */
+int  ngh_block_norm(ngh_context* ctx, const ngh_block_norm_spec* spec);
+/* The statistics are computed again from h and b, so nothing but those two has to be kept from the
+ * forward pass.  Sums over rows are added in a fixed order: the same bits from run to run.       */
+int  ngh_block_norm_grad(ngh_context* ctx, const ngh_block_norm_spec* spec);
+int  ngh_block_norm_grad_workspace(const ngh_block_norm_spec* spec, size_t* out_bytes);
+
+/* AdamW over many tensors at once.  For every element, with t the step and g the gradient times
+ * grad_scale:
+ *     m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2
+ *     p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * A plan holds the addresses of the tensors and is used for every step; the step is one launch.
+ * States are fp32, or 8 bits: every 256 consecutive elements of a tensor (fewer at its end) share an
+ * fp32 scale s, the largest |m| (v) among them, and hold
+ *     m: an int8  q = sign(m) rint(127 sqrt(|m| / s)),  standing for  sign(q) s (q / 127)^2
+ *     v: a uint8  q = rint(255 (v / s)^(1/4)),          standing for  s (q / 255)^4
+ * so that a second moment only becomes 0 where it is below 1.5e-11 of the block's largest.  The
+ * update uses the moments before they are rounded.  A block in which a moment is not finite gets
+ * NaN for its scale: it shows in every element of the block from the next step on.  A tensor that is
+ * written may overlap nothing else of the plan.                                                  */
+#define NGH_ADAMW_BLOCK 256
+typedef struct ngh_adamw_tensor {
+    void*       param;               /* [n], param_dtype; updated in place                       */
+    const void* grad;                /* [n], grad_dtype                                          */
+    void*       m;                   /* [n] fp32, or int8                                        */
+    void*       v;                   /* [n] fp32, or uint8                                       */
+    float*      m_scale;             /* 8 bits: [ceil(n / NGH_ADAMW_BLOCK)]; else NULL           */
+    float*      v_scale;
+    void*       copy;                /* [n], copy_dtype: receives the updated parameters as well
+                                        (an fp32 master's 16-bit copy); NULL: none               */
+    int64_t     n;
+    float       weight_decay;
+    int32_t     reserved;
+} ngh_adamw_tensor;
+typedef struct ngh_adamw_hyper {
+    double  lr, beta1, beta2, eps;   /* (1 - beta and the bias corrections are formed in fp64)   */
+    float   grad_scale;              /* gradients are multiplied by it (1: as they are)          */
+    int32_t step;                    /* t, from 1; not read when dev_step is given               */
+    /* For recorded graphs, whose replays read what the device holds then: */
+    int32_t* dev_step;               /* counts the steps: incremented first, then used as t      */
+    const float* dev_lr;             /* in place of lr                                           */
+    const float* dev_grad_scale;     /* multiplied with grad_scale (a clipping factor)           */
+} ngh_adamw_hyper;
+typedef struct ngh_adamw_plan ngh_adamw_plan;
+/* param_dtype and grad_dtype: NGH_F32, NGH_F16 or NGH_BF16; copy_dtype the same or -1; state_bits 8
+ * or 32.  Tensors of length 0 are allowed.  Allocates on the device and waits for the upload.    */
+int  ngh_validate_adamw(const ngh_adamw_tensor* tensors, int32_t n_tensors, int32_t param_dtype, int32_t grad_dtype,
+                        int32_t copy_dtype, int32_t state_bits);           /* no device needed */
+int  ngh_adamw_plan_create(ngh_context* ctx, const ngh_adamw_tensor* tensors, int32_t n_tensors, int32_t param_dtype,
+                           int32_t grad_dtype, int32_t copy_dtype, int32_t state_bits, ngh_adamw_plan** out);
+int  ngh_adamw_step(ngh_context* ctx, ngh_adamw_plan* plan, const ngh_adamw_hyper* hyper);
+int  ngh_adamw_plan_free(ngh_context* ctx, ngh_adamw_plan* plan);      /* waits for the stream */
+/* n moments in 8 bits as fp32 and back (checkpoints); second: 0 the first moments, 1 the second.  */
+int  ngh_adamw_decode(ngh_context* ctx, float* dev_out, const void* dev_codes, const float* dev_scales, int64_t n,
+                      int32_t second);
+int  ngh_adamw_encode(ngh_context* ctx, void* dev_codes, float* dev_scales, const float* dev_in, int64_t n,
+                      int32_t second);
 
 /* ---- timing (HIP events on the context's stream; used by the bench) ----- */
 int  ngh_timer_begin(ngh_context* ctx);

@@ -1,0 +1,434 @@
+// Kernels of ngh_block_norm / ngh_block_norm_grad: the norms before and after a block fused with its
+// gate and residual.  For a row, with bh = N(b):
+//     u = bh p + q;   h = alpha x + g u;   y = N(h) w + z
+// and backward, with T the transpose of N's Jacobian, T(t; x) = r (t - xh mean(t xh) [- mean(t)]):
+//     d = dh + T(dy w; h);   dx = alpha d;   dg += d u;   e = d g;   dp += e bh;   dq += e;
+//     db = T(e p; b);   dw += dy hh;   dz += dy
+// A row is held in registers as fp32 from its one load on (C chunks of VEC elements a lane, a row on
+// NW wavefronts or, NW = 1, on a power of two of lanes), so the forward pass reads x and b and writes
+// h and y once, the backward pass reads dh, dy, h and b and writes dx and db: both are bound by
+// memory.  The variance of the layer norm is taken around the mean, in registers.  The statistics are
+// computed again in the backward pass: a reduction that is there anyway, and no operand.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "ngh_internal.h"
+#include "ngh_rows.h"
+
+namespace ngh {
+
+struct NormArgs {
+    const void *x, *b, *gain, *bias, *post_gain, *post_bias, *gate, *dy, *dh;
+    void *h, *y, *dx, *db, *dgate;
+    float* parts;                  // backward: [part][vector][part_stride] sums of a part's rows
+    long long x_stride, b_stride, gate_stride, h_stride, y_stride, dy_stride, dh_stride, dx_stride, db_stride, dgate_stride, part_stride;
+    unsigned rows, width, gate_rows;
+    int lanes;                     // NW == 1: lanes along a row
+    int layer, post, param_f32;
+    float eps, alpha, inv_width;
+    // backward: rows [part * per_part, ...) of a span of consecutive rows of one gate row, or several whole ones
+    unsigned span_rows, parts_per_span, per_part;
+    int vectors;                   // sums a part writes: gain, bias, post gain, post bias, gate (bits), in this order
+    int gate_whole;                // a part holds whole gate rows and writes their gradients itself
+};
+
+constexpr int kVecGain = 1, kVecBias = 2, kVecPostGain = 4, kVecPostBias = 8, kVecGate = 16;
+
+// VEC elements of a gain, bias or gate; `other` where there is none.
+template <class T, int VEC, bool RAGGED>
+__device__ __forceinline__ void load_param(const void* p, long long at, int count, bool f32, float other, float (&out)[VEC]) {
+    if (!p) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out[i] = other;
+    } else if (f32) {
+        load_piece<float, VEC, RAGGED>((const float*)p + at, count, out);
+    } else {
+        load_piece<T, VEC, RAGGED>((const T*)p + at, count, out);
+    }
+}
+
+template <class T, int VEC, int C, int NW, bool RAGGED>
+__global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_norm_kernel(NormArgs a) {
+    constexpr int kThreads = NW == 1 ? 256 : NW * 64;
+    __shared__ float sh[NW == 1 ? 1 : 2 * kRowSumsMax * NW];
+    int phase = 0;
+    const unsigned lanes = NW == 1 ? (unsigned)a.lanes : kThreads;
+    const unsigned lane = threadIdx.x & (lanes - 1);
+    const unsigned row = NW == 1 ? blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes : blockIdx.x;
+    const bool live = row < a.rows;                      // (idle lanes still take part in the reductions)
+    const unsigned n = live ? row : 0;
+    float v[C][VEC], x[C][VEC];
+    int in[C];                                           // elements of each piece
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const unsigned col = (c * lanes + lane) * VEC;
+        in[c] = live ? piece_count<VEC, RAGGED>(col, a.width) : 0;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[c][i] = x[c][i] = 0.0f;
+        if (in[c]) {
+            load_piece<T, VEC, RAGGED>((const T*)a.x + (long long)n * a.x_stride + col, in[c], x[c]);
+            if (a.b) load_piece<T, VEC, RAGGED>((const T*)a.b + (long long)n * a.b_stride + col, in[c], v[c]);
+        }
+    }
+    if (a.post) {
+        float mean = 0.0f;
+        if (a.layer) {
+            float s[1] = {0.0f};
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) s[0] += v[c][i];
+            row_sums<1, NW>(s, lanes, sh, phase);
+            mean = s[0] * a.inv_width;
+        }
+        float s[1] = {0.0f};
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                v[c][i] = (RAGGED ? i < in[c] : in[c] > 0) ? v[c][i] - mean : 0.0f;
+                s[0] += v[c][i] * v[c][i];
+            }
+        row_sums<1, NW>(s, lanes, sh, phase);
+        const float r = 1.0f / sqrtf(s[0] * a.inv_width + a.eps);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const unsigned col = (c * lanes + lane) * VEC;
+            float p[VEC], q[VEC];
+            if (in[c]) {
+                load_param<T, VEC, RAGGED>(a.post_gain, col, in[c], a.param_f32, 1.0f, p);
+                load_param<T, VEC, RAGGED>(a.post_bias, col, in[c], a.param_f32, 0.0f, q);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) v[c][i] = v[c][i] * r * p[i] + q[i];
+            }
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const unsigned col = (c * lanes + lane) * VEC;
+        if (in[c]) {
+            float g[VEC];
+            load_param<T, VEC, RAGGED>(a.gate, a.gate ? (long long)(n / a.gate_rows) * a.gate_stride + col : 0, in[c], a.param_f32, 1.0f, g);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[c][i] = a.alpha * x[c][i] + v[c][i] * g[i];
+            if (a.h) store_piece<T, VEC, RAGGED>((T*)a.h + (long long)n * a.h_stride + col, in[c], v[c]);
+        }
+    }
+    if (!a.y) return;
+    float mean = 0.0f;
+    if (a.layer) {
+        float s[1] = {0.0f};
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) s[0] += v[c][i];
+        row_sums<1, NW>(s, lanes, sh, phase);
+        mean = s[0] * a.inv_width;
+    }
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            v[c][i] = (RAGGED ? i < in[c] : in[c] > 0) ? v[c][i] - mean : 0.0f;
+            s[0] += v[c][i] * v[c][i];
+        }
+    row_sums<1, NW>(s, lanes, sh, phase);
+    const float r = 1.0f / sqrtf(s[0] * a.inv_width + a.eps);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const unsigned col = (c * lanes + lane) * VEC;
+        if (in[c]) {
+            float w[VEC], z[VEC];
+            load_param<T, VEC, RAGGED>(a.gain, col, in[c], a.param_f32, 1.0f, w);
+            load_param<T, VEC, RAGGED>(a.bias, col, in[c], a.param_f32, 0.0f, z);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[c][i] = v[c][i] * r * w[i] + z[i];
+            store_piece<T, VEC, RAGGED>((T*)a.y + (long long)n * a.y_stride + col, in[c], v[c]);
+        }
+    }
+}
+
+// Backward.  A workgroup (with NW = 1: each group of lanes of it) takes the rows of a part one after the
+// other and keeps the part's sums over rows in registers; they go to a.parts at its end, and
+// block_norm_merge_kernel adds the parts in order.  BIAS: the sums of dz and dq are wanted.
+template <class T, int VEC, int C, int NW, bool RAGGED, bool BIAS>
+__global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_norm_grad_kernel(NormArgs a) {
+    constexpr int kThreads = NW == 1 ? 256 : NW * 64;
+    __shared__ float sh[NW == 1 ? 1 : 2 * kRowSumsMax * NW];
+    int phase = 0;
+    const unsigned lanes = NW == 1 ? (unsigned)a.lanes : kThreads;
+    const unsigned lane = threadIdx.x & (lanes - 1);
+    const unsigned part = NW == 1 ? blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes : blockIdx.x;
+    const unsigned span = part / a.parts_per_span;
+    const unsigned first = span * a.span_rows + (part - span * a.parts_per_span) * a.per_part;
+    const unsigned span_end = min(a.rows, (span + 1) * a.span_rows);
+    const unsigned last = first < span_end ? min(span_end, first + a.per_part) : first;
+    // (every group of lanes of a workgroup makes the same number of turns)
+    float sw[C][VEC], sp[C][VEC], sg[C][VEC], sz[BIAS ? C : 1][VEC], sq[BIAS ? C : 1][VEC];
+    int in[C];                                           // elements of each piece
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        in[c] = piece_count<VEC, RAGGED>((c * lanes + lane) * VEC, a.width);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            sw[c][i] = sp[c][i] = sg[c][i] = 0.0f;
+            if constexpr (BIAS) sz[c][i] = sq[c][i] = 0.0f;
+        }
+    }
+    for (unsigned turn = 0; turn < a.per_part; ++turn) {
+        const bool live = first + turn < last;
+        if constexpr (NW > 1) {
+            if (!live) break;
+        }
+        const unsigned n = live ? first + turn : 0;
+        float h[C][VEC], b[C][VEC], d[C][VEC], t[C][VEC];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const unsigned col = (c * lanes + lane) * VEC;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) h[c][i] = b[c][i] = d[c][i] = t[c][i] = 0.0f;
+            if (live && in[c]) {
+                if (a.dy) {
+                    load_piece<T, VEC, RAGGED>((const T*)a.h + (long long)n * a.h_stride + col, in[c], h[c]);
+                    load_piece<T, VEC, RAGGED>((const T*)a.dy + (long long)n * a.dy_stride + col, in[c], t[c]);
+                }
+                if (a.b) load_piece<T, VEC, RAGGED>((const T*)a.b + (long long)n * a.b_stride + col, in[c], b[c]);
+                if (a.dh) load_piece<T, VEC, RAGGED>((const T*)a.dh + (long long)n * a.dh_stride + col, in[c], d[c]);
+            }
+        }
+        float bmean = 0.0f, brs = 1.0f;
+        // the norm after the block: its statistics, and d
+        if (a.layer) {
+            float s[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    s[0] += h[c][i];
+                    s[1] += b[c][i];
+                }
+            row_sums<2, NW>(s, lanes, sh, phase);
+            const float hmean = s[0] * a.inv_width;
+            bmean = a.post ? s[1] * a.inv_width : 0.0f;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    h[c][i] = (RAGGED ? i < in[c] : in[c] > 0) ? h[c][i] - hmean : 0.0f;
+                    b[c][i] = (RAGGED ? i < in[c] : in[c] > 0) ? b[c][i] - bmean : 0.0f;
+                }
+        }
+        {
+            // sums of h^2, t h and t (t = dy w), b^2
+            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float w[VEC];
+                const unsigned col = (c * lanes + lane) * VEC;
+                if (live && in[c]) {
+                    load_param<T, VEC, RAGGED>(a.gain, col, in[c], a.param_f32, 1.0f, w);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) w[i] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float tw = t[c][i] * w[i];
+                    s[0] += h[c][i] * h[c][i];
+                    s[1] += tw * h[c][i];
+                    s[2] += tw;
+                    s[3] += b[c][i] * b[c][i];
+                }
+            }
+            row_sums<4, NW>(s, lanes, sh, phase);
+            const float r = 1.0f / sqrtf(s[0] * a.inv_width + a.eps);
+            if (a.post) brs = 1.0f / sqrtf(s[3] * a.inv_width + a.eps);
+            if (a.dy) {
+                const float along = s[1] * r * a.inv_width;              // mean(t hh)
+                const float level = a.layer ? s[2] * a.inv_width : 0.0f;
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    float w[VEC];
+                    const unsigned col = (c * lanes + lane) * VEC;
+                    if (live && in[c]) {
+                        load_param<T, VEC, RAGGED>(a.gain, col, in[c], a.param_f32, 1.0f, w);
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) {
+                            const float hh = h[c][i] * r;
+                            sw[c][i] += t[c][i] * hh;
+                            if constexpr (BIAS) sz[c][i] += t[c][i];
+                            if (!RAGGED || i < in[c]) d[c][i] += r * (t[c][i] * w[i] - hh * along - level);
+                        }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const unsigned col = (c * lanes + lane) * VEC;
+            if (live && in[c] && a.dx) {
+                float o[VEC];
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) o[i] = a.alpha * d[c][i];
+                store_piece<T, VEC, RAGGED>((T*)a.dx + (long long)n * a.dx_stride + col, in[c], o);
+            }
+        }
+        if (!a.db) continue;
+        const unsigned gate_row = a.gate ? n / a.gate_rows : 0;
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const unsigned col = (c * lanes + lane) * VEC;
+            if (live && in[c]) {
+                float g[VEC], p[VEC], q[VEC];
+                load_param<T, VEC, RAGGED>(a.gate, a.gate ? (long long)gate_row * a.gate_stride + col : 0, in[c], a.param_f32, 1.0f, g);
+                load_param<T, VEC, RAGGED>(a.post_gain, col, in[c], a.param_f32, 1.0f, p);
+                load_param<T, VEC, RAGGED>(a.post_bias, col, in[c], a.param_f32, 0.0f, q);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float bh = b[c][i] * brs;
+                    b[c][i] = bh;
+                    sg[c][i] += d[c][i] * (bh * p[i] + q[i]);
+                    const float e = d[c][i] * g[i];
+                    sp[c][i] += e * bh;
+                    if constexpr (BIAS) sq[c][i] += e;
+                    d[c][i] = e * p[i];
+                    s[0] += d[c][i] * bh;
+                    s[1] += d[c][i];
+                }
+            }
+        }
+        if (a.post) {
+            row_sums<2, NW>(s, lanes, sh, phase);
+            const float along = s[0] * a.inv_width, level = a.layer ? s[1] * a.inv_width : 0.0f;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) d[c][i] = brs * (d[c][i] - b[c][i] * along - level);
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const unsigned col = (c * lanes + lane) * VEC;
+            if (live && in[c]) store_piece<T, VEC, RAGGED>((T*)a.db + (long long)n * a.db_stride + col, in[c], d[c]);
+        }
+        if (a.gate_whole && a.dgate && (n + 1) % a.gate_rows == 0) {
+            // the last row of a gate row: its gradient is complete
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const unsigned col = (c * lanes + lane) * VEC;
+                if (live && in[c]) {
+                    const long long at = (long long)gate_row * a.dgate_stride + col;
+                    if (a.param_f32) store_piece<float, VEC, RAGGED>((float*)a.dgate + at, in[c], sg[c]);
+                    else store_piece<T, VEC, RAGGED>((T*)a.dgate + at, in[c], sg[c]);
+                }
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) sg[c][i] = live ? 0.0f : sg[c][i];
+            }
+        }
+    }
+    if (!a.vectors || first >= span_end) return;
+    float* out = a.parts + (size_t)part * __popc(a.vectors) * a.part_stride;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const unsigned col = (c * lanes + lane) * VEC;
+        if (!in[c]) continue;
+        float* to = out + col;
+        if (a.vectors & kVecGain) store_from_float<float, VEC>(to, sw[c]), to += a.part_stride;
+        if constexpr (BIAS) {
+            if (a.vectors & kVecBias) store_from_float<float, VEC>(to, sz[c]), to += a.part_stride;
+        }
+        if (a.vectors & kVecPostGain) store_from_float<float, VEC>(to, sp[c]), to += a.part_stride;
+        if constexpr (BIAS) {
+            if (a.vectors & kVecPostBias) store_from_float<float, VEC>(to, sq[c]), to += a.part_stride;
+        }
+        if (a.vectors & kVecGate) store_from_float<float, VEC>(to, sg[c]);
+    }
+}
+
+struct NormMergeArgs {
+    const float* parts;
+    long long part_stride;
+    unsigned width, per_part_vectors, n_parts, parts_per_span, gates;            // gates: 1 when the last vector is the gate's
+    unsigned first;                // of the sums this launch makes (its grid's second axis is limited)
+    void* out[4];                  // of the vectors other than the gate
+    void* dgate;
+    long long dgate_stride;
+};
+
+// Sums the parts of a vector (over all of them) or of a gate row (over those of its span): 64 columns a
+// workgroup, 16 wavefronts each adding a run of parts, joined in LDS in that order.
+template <class T>
+__global__ __launch_bounds__(1024) void block_norm_merge_kernel(NormMergeArgs a) {
+    __shared__ float sh[16][64];
+    const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const unsigned col = blockIdx.x * 64 + lane;
+    const unsigned plain = a.per_part_vectors - a.gates;
+    const unsigned which = a.first + blockIdx.y;
+    const bool gate = which >= plain;
+    const unsigned vec = gate ? plain : which, span = gate ? which - plain : 0;
+    const unsigned begin = gate ? span * a.parts_per_span : 0;
+    const unsigned count = gate ? a.parts_per_span : a.n_parts;
+    const unsigned share = (count + 15) / 16;
+    const unsigned p0 = min(count, wave * share), p1 = min(count, p0 + share);
+    const float* from = a.parts + ((size_t)begin * a.per_part_vectors + vec) * a.part_stride + col;
+    const size_t step = (size_t)a.per_part_vectors * a.part_stride;
+    float acc = 0.0f;
+    if (col < a.width)
+        for (unsigned p = p0; p < p1; p += 8) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = p + k < p1 ? from[(p + k) * step] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc += v[k];
+        }
+    sh[wave][lane] = acc;
+    __syncthreads();
+    if (wave != 0 || col >= a.width) return;
+#pragma unroll
+    for (int w = 1; w < 16; ++w) acc += sh[w][lane];
+    if (gate) ((T*)a.dgate)[(long long)span * a.dgate_stride + col] = (T)acc;
+    else ((T*)a.out[vec])[col] = (T)acc;
+}
+
+// The shape of the kernel that a row takes: C pieces of VEC elements a lane, `waves` wavefronts (one: `lanes`
+// lanes of it).  ragged: rows that do not start, or end, on 16-byte boundaries.
+struct NormShape {
+    int pieces, waves, lanes;
+    bool ragged;
+};
+
+// One translation unit for each storage type; `backward` chooses the kernel.
+NGH_INTERNAL int launch_norm_f32(const NormShape& s, const NormArgs& a, bool backward, bool bias, unsigned grid, hipStream_t stream);
+NGH_INTERNAL int launch_norm_f16(const NormShape& s, const NormArgs& a, bool backward, bool bias, unsigned grid, hipStream_t stream);
+NGH_INTERNAL int launch_norm_bf16(const NormShape& s, const NormArgs& a, bool backward, bool bias, unsigned grid, hipStream_t stream);
+
+template <class T, int VEC, int C, int NW, bool RAGGED>
+void launch_norm_kernel(const NormArgs& a, bool backward, bool bias, unsigned grid, hipStream_t stream) {
+    const dim3 block(NW == 1 ? 256 : NW * 64);
+    if (!backward) hipLaunchKernelGGL((block_norm_kernel<T, VEC, C, NW, RAGGED>), dim3(grid), block, 0, stream, a);
+    else if (bias) hipLaunchKernelGGL((block_norm_grad_kernel<T, VEC, C, NW, RAGGED, true>), dim3(grid), block, 0, stream, a);
+    else hipLaunchKernelGGL((block_norm_grad_kernel<T, VEC, C, NW, RAGGED, false>), dim3(grid), block, 0, stream, a);
+}
+
+// 8 elements a lane on up to 8 wavefronts (rows of up to 4096 elements), 16 on 8 or 16.
+template <class T, bool RAGGED>
+int launch_norm(const NormShape& s, const NormArgs& a, bool backward, bool bias, unsigned grid, hipStream_t stream) {
+    constexpr int kVec = 16 / sizeof(T), kEight = 8 / kVec;
+    if (s.pieces == kEight) {
+        switch (s.waves) {
+            case 1: launch_norm_kernel<T, kVec, kEight, 1, RAGGED>(a, backward, bias, grid, stream); break;
+            case 2: launch_norm_kernel<T, kVec, kEight, 2, RAGGED>(a, backward, bias, grid, stream); break;
+            case 4: launch_norm_kernel<T, kVec, kEight, 4, RAGGED>(a, backward, bias, grid, stream); break;
+            default: launch_norm_kernel<T, kVec, kEight, 8, RAGGED>(a, backward, bias, grid, stream); break;
+        }
+    } else if (s.waves == 8) {
+        launch_norm_kernel<T, kVec, 2 * kEight, 8, RAGGED>(a, backward, bias, grid, stream);
+    } else {
+        launch_norm_kernel<T, kVec, 2 * kEight, 16, RAGGED>(a, backward, bias, grid, stream);
+    }
+    NGH_HIP_TRY(hipGetLastError());
+    return NGH_OK;
+}
+
+}  // namespace ngh

@@ -1,0 +1,292 @@
+// ngh_block_norm, ngh_block_norm_grad: checks, the shape of the kernels and the launches.  The
+// mathematics and the kernels are in ngh_block_norm.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "ngh_block_norm.h"
+
+namespace ngh {
+namespace {
+
+int size_of(int dtype) { return dtype == NGH_F32 ? 4 : (dtype == NGH_F16 || dtype == NGH_BF16) ? 2 : 0; }
+
+struct View {
+    const char* name;
+    const void* p;
+    int64_t rows, stride;
+    int item;
+    bool written;
+};
+
+constexpr int kMostViews = 20;
+
+// Everything the call touches; returns how many.
+int views_of(const ngh_block_norm_spec* s, bool grad, View (&v)[kMostViews]) {
+    const int e = size_of(s->dtype), q = size_of(s->param_dtype);
+    const int64_t gates = s->gate_rows > 0 ? s->rows / s->gate_rows : 0;
+    int n = 0;
+    auto add = [&](const char* name, const void* p, int64_t rows, int64_t stride, int item, bool written) {
+        if (p) v[n++] = View{name, p, rows, stride, item, written};
+    };
+    add("gain", s->gain, 1, s->width, q, false);
+    add("post_gain", s->post_gain, 1, s->width, q, false);
+    add("post_bias", s->post_bias, 1, s->width, q, false);
+    add("gate", s->gate, gates, s->gate_stride, q, false);
+    add("b", s->b, s->rows, s->b_stride, e, false);
+    add("h", s->h, s->rows, s->h_stride, e, !grad);
+    if (!grad) {
+        add("bias", s->bias, 1, s->width, q, false);
+        add("x", s->x, s->rows, s->x_stride, e, false);
+        add("y", s->y, s->rows, s->y_stride, e, true);
+    } else {
+        add("dy", s->dy, s->rows, s->dy_stride, e, false);
+        add("dh", s->dh, s->rows, s->dh_stride, e, false);
+        add("dx", s->dx, s->rows, s->dx_stride, e, true);
+        add("db", s->db, s->rows, s->db_stride, e, true);
+        add("dgain", s->dgain, 1, s->width, q, true);
+        add("dbias", s->dbias, 1, s->width, q, true);
+        add("dpost_gain", s->dpost_gain, 1, s->width, q, true);
+        add("dpost_bias", s->dpost_bias, 1, s->width, q, true);
+        add("dgate", s->dgate, gates, s->dgate_stride, q, true);
+        add("workspace", s->workspace, 1, (int64_t)s->workspace_bytes, 1, true);
+    }
+    return n;
+}
+
+int check(const ngh_block_norm_spec* s, bool grad, const char* what) {
+    if (!s) return report(NGH_E_INVALID, "%s: spec is NULL", what);
+    if (s->abi_version != NGH_ABI_VERSION)
+        return report(NGH_E_INVALID, "%s: abi_version %d, this library is %d", what, s->abi_version, NGH_ABI_VERSION);
+    if (s->kind != NGH_NORM_RMS && s->kind != NGH_NORM_LAYER) return report(NGH_E_INVALID, "%s: kind %d", what, s->kind);
+    if (!size_of(s->dtype) || (s->param_dtype != s->dtype && s->param_dtype != NGH_F32))
+        return report(NGH_E_INVALID, "%s: dtype %d with parameters of dtype %d (NGH_F32, NGH_F16, NGH_BF16; parameters the same or NGH_F32)", what,
+                      s->dtype, s->param_dtype);
+    if (s->rows < 0 || s->width < 1) return report(NGH_E_INVALID, "%s: rows %lld, width %lld", what, (long long)s->rows, (long long)s->width);
+    if (s->width > NGH_BLOCK_NORM_MAX_WIDTH || s->rows >= (1LL << 31) - 65536)
+        return report(NGH_E_UNSUPPORTED, "%s: %lld rows of %lld elements", what, (long long)s->rows, (long long)s->width);
+    if (!(s->eps >= 0.0f) || !std::isfinite(s->eps) || !std::isfinite(s->residual_scale))
+        return report(NGH_E_INVALID, "%s: eps %g, residual_scale %g", what, (double)s->eps, (double)s->residual_scale);
+    const bool block = s->b != nullptr || (grad && s->db != nullptr);
+    if (!block && (s->post_norm || s->post_gain || s->post_bias || s->gate))
+        return report(NGH_E_INVALID, "%s: a norm, gain, bias or gate after the block, and no block output", what);
+    if (!s->post_norm && (s->post_gain || s->post_bias))
+        return report(NGH_E_INVALID, "%s: a gain or bias after the block without post_norm", what);
+    if (s->gate) {
+        if (s->gate_rows < 1 || s->rows % s->gate_rows) return report(NGH_E_INVALID, "%s: gate_rows %lld of %lld rows", what, (long long)s->gate_rows, (long long)s->rows);
+    } else if (s->gate_rows) {
+        return report(NGH_E_INVALID, "%s: gate_rows without a gate", what);
+    }
+    if (!grad) {
+        if (!s->x && s->rows) return report(NGH_E_INVALID, "%s: x is NULL", what);
+        if (!s->h && !s->y && s->rows) return report(NGH_E_INVALID, "%s: neither h nor y", what);
+        if (!s->y && (s->gain || s->bias)) return report(NGH_E_INVALID, "%s: a gain or bias without y", what);
+    } else if (s->rows) {
+        if (!s->dy && !s->dh) return report(NGH_E_INVALID, "%s: neither dy nor dh", what);
+        if (s->dy && !s->h) return report(NGH_E_INVALID, "%s: dy without h", what);
+        if ((s->b != nullptr) != (s->db != nullptr)) return report(NGH_E_INVALID, "%s: b and db come together", what);
+        if (!s->dx && !s->db) return report(NGH_E_INVALID, "%s: neither dx nor db", what);
+        if (!s->dy && (s->gain || s->dgain || s->dbias)) return report(NGH_E_INVALID, "%s: the gain or its gradient without dy", what);
+        if (!s->post_norm && (s->dpost_gain || s->dpost_bias)) return report(NGH_E_INVALID, "%s: a gradient of the norm after the block without post_norm", what);
+        if (s->dgate && !s->gate) return report(NGH_E_INVALID, "%s: dgate without a gate", what);
+    }
+    View v[kMostViews];
+    const int n = views_of(s, grad, v);
+    for (int i = 0; i < n; ++i) {
+        if ((uintptr_t)v[i].p % v[i].item) return report(NGH_E_INVALID, "%s: %s is not aligned to its elements", what, v[i].name);
+        if (v[i].rows > 1 && v[i].stride < s->width) return report(NGH_E_INVALID, "%s: stride %lld of %s below the width", what, (long long)v[i].stride, v[i].name);
+        if (v[i].stride >= (1LL << 40)) return report(NGH_E_UNSUPPORTED, "%s: stride of %s too large", what, v[i].name);
+    }
+    auto bytes = [&](const View& a) {
+        return a.item == 1 ? (unsigned long long)a.stride : span_bytes(a.rows, s->width, a.stride, a.item);      // (item 1: the workspace)
+    };
+    for (int i = 0; i < n; ++i)
+        for (int j = 0; j < n; ++j) {
+            if (i == j || !v[i].written || (v[j].written && j < i)) continue;
+            if (!spans_overlap(v[i].p, bytes(v[i]), v[j].p, bytes(v[j]))) continue;
+            // a row is read whole before it is written: the stream and its gradient may be updated in place
+            const bool same = v[i].p == v[j].p && (v[i].stride == v[j].stride || s->rows == 1);
+            if (same && ((v[i].p == s->h && v[j].p == s->x && !grad && v[j].p != s->b) || (grad && v[i].p == s->dx && v[j].p == s->dh))) continue;
+            return report(NGH_E_INVALID, "%s: %s overlaps %s", what, v[i].name, v[j].name);
+        }
+    return NGH_OK;
+}
+
+NormShape shape_of(const ngh_block_norm_spec* s, bool grad) {
+    NormShape f;
+    View v[kMostViews];
+    const int n = views_of(s, grad, v);
+    const int vec = 16 / size_of(s->dtype);
+    bool whole = s->width % vec == 0;
+    for (int i = 0; i < n; ++i) {
+        if (v[i].item == 1) continue;
+        const int piece = std::min(16, vec * v[i].item);
+        whole = whole && (uintptr_t)v[i].p % piece == 0 && (v[i].rows <= 1 || v[i].stride * v[i].item % piece == 0);
+    }
+    f.ragged = !whole;
+    const int per_lane = s->width > 8 * 64 * 8 ? 16 : 8;
+    f.pieces = per_lane / vec;
+    f.lanes = 1;
+    while (f.lanes < 64 && f.lanes * per_lane < s->width) f.lanes *= 2;
+    f.waves = 1;
+    while (f.waves * 64 * per_lane < s->width) f.waves *= 2;
+    return f;
+}
+
+void fill_args(const ngh_block_norm_spec* s, const NormShape& f, NormArgs& a) {
+    a = NormArgs{};
+    a.x = s->x, a.b = s->b, a.gain = s->gain, a.bias = s->bias, a.post_gain = s->post_gain, a.post_bias = s->post_bias, a.gate = s->gate;
+    a.dy = s->dy, a.dh = s->dh, a.h = s->h, a.y = s->y, a.dx = s->dx, a.db = s->db, a.dgate = s->dgate;
+    a.x_stride = s->x_stride, a.b_stride = s->b_stride, a.gate_stride = s->gate_stride, a.h_stride = s->h_stride, a.y_stride = s->y_stride;
+    a.dy_stride = s->dy_stride, a.dh_stride = s->dh_stride, a.dx_stride = s->dx_stride, a.db_stride = s->db_stride, a.dgate_stride = s->dgate_stride;
+    a.rows = (unsigned)s->rows;
+    a.width = (unsigned)s->width;
+    a.gate_rows = (unsigned)std::max<int64_t>(1, s->gate_rows);
+    a.lanes = f.lanes;
+    a.layer = s->kind == NGH_NORM_LAYER;
+    a.post = s->post_norm != 0;
+    a.param_f32 = s->param_dtype == NGH_F32;
+    a.eps = s->eps;
+    a.alpha = s->residual_scale;
+    a.inv_width = 1.0f / (float)s->width;
+}
+
+int launch(const ngh_block_norm_spec* s, const NormShape& f, const NormArgs& a, bool backward, bool bias, unsigned grid, hipStream_t stream) {
+    if (s->dtype == NGH_F32) return launch_norm_f32(f, a, backward, bias, grid, stream);
+    if (s->dtype == NGH_F16) return launch_norm_f16(f, a, backward, bias, grid, stream);
+    return launch_norm_bf16(f, a, backward, bias, grid, stream);
+}
+
+// How the rows of the backward pass are dealt, and where the sums of the parts lie.
+struct GradPlan {
+    NormShape shape;
+    unsigned span_rows, spans, parts_per_span, per_part, parts, grid;
+    int vectors, count;
+    bool gate_whole, bias;
+    size_t part_stride, bytes;
+};
+
+GradPlan plan_grad(const ngh_block_norm_spec* s, int cus) {
+    GradPlan g;
+    g.shape = shape_of(s, true);
+    g.vectors = (s->dgain ? kVecGain : 0) | (s->dbias ? kVecBias : 0) | (s->dpost_gain ? kVecPostGain : 0) | (s->dpost_bias ? kVecPostBias : 0);
+    g.bias = s->dbias || s->dpost_bias;
+    const unsigned rows = (unsigned)s->rows;
+    // Two workgroups a compute unit, but at least 8 rows a part: a part's sums are written in fp32 and
+    // read once more.
+    const unsigned groups = g.shape.waves == 1 ? 256u / g.shape.lanes : 1u;              // parts a workgroup holds
+    const unsigned want = 2u * cus * groups;
+    g.per_part = std::max(8u, (rows + want - 1) / std::max(1u, want));
+    const unsigned gate_rows = (unsigned)std::max<int64_t>(1, s->gate_rows);
+    g.gate_whole = !s->dgate || gate_rows < 2 * g.per_part;
+    g.span_rows = g.gate_whole ? std::max(1u, rows) : gate_rows;
+    if (!g.gate_whole) {
+        // the rows of a gate row are shared by as many parts as they fill
+        g.vectors |= kVecGate;
+        const unsigned parts = gate_rows / g.per_part;
+        g.per_part = (gate_rows + parts - 1) / parts;
+    } else if (s->dgate) {
+        g.per_part = std::max(1u, g.per_part / gate_rows) * gate_rows;                   // (whole gate rows)
+    }
+    g.count = __builtin_popcount((unsigned)g.vectors);
+    g.spans = g.gate_whole ? 1 : rows / g.span_rows;
+    g.parts_per_span = (g.span_rows + g.per_part - 1) / g.per_part;
+    g.parts = g.spans * g.parts_per_span;
+    g.grid = (g.parts + groups - 1) / groups;
+    g.part_stride = ((size_t)s->width + 7) / 8 * 8;
+    g.bytes = (size_t)g.parts * g.count * g.part_stride * 4;
+    return g;
+}
+
+template <class T>
+int launch_merge(NormMergeArgs m, unsigned spans, hipStream_t stream) {
+    const unsigned sums = m.per_part_vectors - m.gates + (m.gates ? spans : 0);
+    for (m.first = 0; m.first < sums; m.first += 65535u) {
+        hipLaunchKernelGGL(block_norm_merge_kernel<T>, dim3((m.width + 63) / 64, std::min(65535u, sums - m.first)), dim3(1024), 0, stream, m);
+        NGH_HIP_TRY(hipGetLastError());
+    }
+    return NGH_OK;
+}
+
+}  // namespace
+}  // namespace ngh
+
+using namespace ngh;
+
+extern "C" {
+
+int ngh_validate_block_norm(const ngh_block_norm_spec* spec, int32_t gradient) {
+    return check(spec, gradient != 0, gradient ? "ngh_block_norm_grad" : "ngh_block_norm");
+}
+
+int ngh_block_norm(ngh_context* ctx, const ngh_block_norm_spec* spec) {
+    const int rc = ctx ? check(spec, false, "ngh_block_norm") : report(NGH_E_INVALID, "ctx is NULL");
+    if (rc != NGH_OK || spec->rows == 0) return rc;
+    const ContextView c = view_of(ctx);
+    DeviceScope scope(c.device);
+    if (!scope.ok()) return report(NGH_E_RUNTIME, "ngh_block_norm: the context's device cannot be made current");
+    const NormShape f = shape_of(spec, false);
+    NormArgs a;
+    fill_args(spec, f, a);
+    const unsigned per_wg = f.waves == 1 ? 256u / f.lanes : 1u;
+    return launch(spec, f, a, false, false, (a.rows + per_wg - 1) / per_wg, c.stream);
+}
+
+int ngh_block_norm_grad_workspace(const ngh_block_norm_spec* spec, size_t* out_bytes) {
+    if (!out_bytes) return report(NGH_E_INVALID, "ngh_block_norm_grad_workspace: out_bytes is NULL");
+    *out_bytes = 0;
+    const int rc = check(spec, true, "ngh_block_norm_grad_workspace");
+    if (rc != NGH_OK) return rc;
+    // (how the rows are dealt depends on the device's compute units; enough for any number of them)
+    size_t most = 256;
+    for (int cus = 1; spec->rows && cus <= 1024; cus *= 2) most = std::max(most, plan_grad(spec, cus).bytes);
+    *out_bytes = most;
+    return NGH_OK;
+}
+
+int ngh_block_norm_grad(ngh_context* ctx, const ngh_block_norm_spec* spec) {
+    const int rc = ctx ? check(spec, true, "ngh_block_norm_grad") : report(NGH_E_INVALID, "ctx is NULL");
+    if (rc != NGH_OK) return rc;
+    const ContextView c = view_of(ctx);
+    DeviceScope scope(c.device);
+    if (!scope.ok()) return report(NGH_E_RUNTIME, "ngh_block_norm_grad: the context's device cannot be made current");
+    const GradPlan g = plan_grad(spec, c.cus);
+    if (spec->workspace_bytes < g.bytes || (g.bytes && !spec->workspace))
+        return report(NGH_E_INVALID, "ngh_block_norm_grad: workspace of %zu bytes, %zu needed", spec->workspace_bytes, g.bytes);
+    if ((uintptr_t)spec->workspace % 16) return report(NGH_E_INVALID, "ngh_block_norm_grad: misaligned workspace");
+    NormArgs a;
+    fill_args(spec, g.shape, a);
+    a.parts = (float*)spec->workspace;
+    a.part_stride = (long long)g.part_stride;
+    a.span_rows = g.span_rows;
+    a.parts_per_span = g.parts_per_span;
+    a.per_part = g.per_part;
+    a.vectors = g.vectors;
+    a.gate_whole = g.gate_whole;
+    if (spec->rows) {
+        const int lrc = launch(spec, g.shape, a, true, g.bias, g.grid, c.stream);
+        if (lrc != NGH_OK) return lrc;
+    }
+    if (!g.vectors) return NGH_OK;
+    NormMergeArgs m{};
+    m.parts = a.parts;
+    m.part_stride = a.part_stride;
+    m.width = a.width;
+    m.per_part_vectors = (unsigned)g.count;
+    m.n_parts = spec->rows ? g.parts : 0;
+    m.parts_per_span = g.parts_per_span;
+    m.gates = g.vectors & kVecGate ? 1 : 0;
+    int k = 0;
+    if (spec->dgain) m.out[k++] = spec->dgain;
+    if (spec->dbias) m.out[k++] = spec->dbias;
+    if (spec->dpost_gain) m.out[k++] = spec->dpost_gain;
+    if (spec->dpost_bias) m.out[k++] = spec->dpost_bias;
+    m.dgate = spec->dgate;
+    m.dgate_stride = spec->dgate_stride;
+    if (spec->param_dtype == NGH_F32) return launch_merge<float>(m, g.spans, c.stream);
+    if (spec->param_dtype == NGH_F16) return launch_merge<f16_t>(m, g.spans, c.stream);
+    return launch_merge<bf16_t>(m, g.spans, c.stream);
+}
+
+}  // extern "C"

@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "ngraph_hip.h"
+#include "ngh_internal.h"
 #include "ngh_device.h"
 #include "ngh_interp.h"
 #include "ngh_copy.h"
@@ -159,6 +160,23 @@ struct ngh_context {
     char        name[256] = "";
     uint64_t    total_bytes = 0;
 };
+
+// ---------------------------------------------------------------------------
+// what the other translation units see of a context (ngh_internal.h)
+// ---------------------------------------------------------------------------
+namespace ngh {
+ContextView view_of(const ngh_context* ctx) {
+    return ContextView{ctx->stream, ctx->device, ctx->cus, ctx->capturing};
+}
+
+int report(int code, const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+}  // namespace ngh
 
 // ---------------------------------------------------------------------------
 // spec validation (host only; also run before every launch so a malformed

@@ -12,6 +12,8 @@ import os
 
 import numpy as np
 
+from ngraph_hip.runtime import row_ops
+
 NGH_ABI_VERSION = 7
 NGH_MAX_AXES = 3
 NGH_MAX_TENSORS = 12
@@ -23,6 +25,7 @@ NGH_MAX_STAGES = 6
 
 NGH_F32, NGH_FLEX16, NGH_I32, NGH_F16 = 0, 1, 2, 3
 NGH_U32, NGH_I16, NGH_I8, NGH_U8 = 4, 5, 6, 7
+NGH_BF16 = 8                 # embedding, block norm, AdamW (held as uint16 on the host)
 NGH_SPEC_PROBE = 1
 NGH_CACHE_STREAM_LOAD, NGH_CACHE_STREAM_STORE = 1, 2
 
@@ -154,6 +157,7 @@ _SYMBOLS = {
     "ngh_timer_begin": [_vp],
     "ngh_timer_end": [_vp, ctypes.POINTER(ctypes.c_float)],
 }
+_SYMBOLS.update(row_ops.SYMBOLS)
 
 NGH_PROGRAM_KERNEL_SLOTS = 12
 
@@ -295,7 +299,7 @@ def read_code_bundle(path):
 
 
 _NP_DTYPES = {NGH_F32: np.float32, NGH_FLEX16: np.int16, NGH_I32: np.int32, NGH_F16: np.float16,
-              NGH_U32: np.uint32, NGH_I16: np.int16, NGH_I8: np.int8, NGH_U8: np.uint8}
+              NGH_U32: np.uint32, NGH_I16: np.int16, NGH_I8: np.int8, NGH_U8: np.uint8, NGH_BF16: np.uint16}
 
 
 class DeviceArray(object):
@@ -328,8 +332,13 @@ class DeviceArray(object):
             self.ptr = None
 
 
-class HipRuntime(object):
+class HipRuntime(row_ops.OperatorCalls):
     """One device context: stream, allocations, launches."""
+
+    abi_version = NGH_ABI_VERSION
+
+    def _check(self, rc):
+        _check(self.lib, rc)
 
     def __init__(self, device_id=0):
         self.lib = load_library()
