@@ -4,16 +4,19 @@
 // Lookup: y[n, :] = scale * table[tokens[n], :].  Two streams, nothing else: bound by memory.
 //
 // Gradient: table[v, :] (+)= scale * sum of dy[n, :] over the n with tokens[n] == v.  The order of
-// the sum must not depend on the schedule, so the places n are sorted by (token, n) first:
-//   1. sort.  The token's bits as digits, least significant first, each pass stable.  Up to
-//      kOneSortMax places one workgroup sorts in LDS (one launch); more are dealt in tiles of
-//      kTile places, a pass being one launch that ranks and scatters (the digit counts of the next
-//      pass are taken while scattering).  In the first launch all other workgroups fill the table
-//      with zeros, which is most of the traffic of an ordinary step and hides the sort.
+// the sum must not depend on the schedule.  Up to kFew places one launch does everything: a wavefront
+// for each place looks through all tokens, goes on if none before it is the same, and adds the rows of
+// its token in order of their places (its whole workgroup does where there are many); other workgroups
+// clear the rows of the table whose token does not occur.  More places are sorted by (token, place) first:
+//   1. sort.  Up to kRankMax places: chunks of kChunk are ranked by all pairs, then every place looks
+//      its rank up in the other chunks.  More: tiles of kTile places, sorted by the token's bits as
+//      digits, least significant first, each pass stable: a launch that counts a tile's digits and one
+//      that ranks and scatters.
 //   2. sums.  The sorted list is cut into units of equal length, whatever the tokens are: a unit is
 //      summed by a wavefront for each block of columns, row after row in fp32.  A token all of whose
 //      rows lie in one unit is finished there; parts of a token that crosses units go to the
 //      workspace, so that one frequent token is spread over as many wavefronts as many rare ones.
+//      In the same launch other workgroups clear the rows whose token the sorted list does not hold.
 //   3. merge.  A workgroup for each unit in which a crossing token begins adds its parts in order.
 #include <hip/hip_runtime.h>
 
@@ -28,9 +31,12 @@ namespace {
 constexpr int kEmbBlock = 256;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / 64;
-constexpr int kItems = 16;                               // places a lane of the one-workgroup sort holds
-constexpr int kOneSortMax = kSortThreads * kItems;       // 16384: keys and places take 96 KiB of LDS
-constexpr int kOneDigitBits = 6;
+constexpr int kRankMax = 16384;                          // places sorted by chunks: 64 KiB of keys in LDS
+constexpr int kChunk = 2048;
+constexpr int kFew = 2048;                               // places that need no sort
+constexpr int kFewWaves = 8;
+constexpr int kFewAlone = 16;                            // rows a wavefront adds by itself (one batch in flight)
+constexpr int kFewRows = 4096;                           // rows of the table one workgroup clears at most
 constexpr int kTileItems = 4;
 constexpr int kTile = kSortThreads * kTileItems;
 constexpr int kTileDigitBits = 9;
@@ -96,14 +102,13 @@ struct SortArgs {
     const int32_t* tokens;
     unsigned n, vocab;
     int pad;
-    unsigned* key_in;      // sorted so far (tiles, passes after the first)
-    unsigned* place_in;
+    const unsigned* key_in;      // sorted so far (tiles, passes after the first)
+    const unsigned* place_in;
     unsigned* key_out;
     unsigned* place_out;
-    unsigned* table;       // [tiles][kTileDigits] counts of this pass
-    unsigned* next;        // ... of the next pass; NULL in the last
+    unsigned* table;             // [tiles][kTileDigits] counts of this pass
     unsigned tiles;
-    int shift, bits, next_shift, next_bits;
+    int shift, bits;
 };
 
 // A token that takes part in no sum sorts behind all others.
@@ -139,177 +144,157 @@ __device__ __forceinline__ unsigned scan_exclusive(unsigned v, unsigned* sh) {
     return before + s - v;
 }
 
-// The part of the table that workgroup `part` of `parts` clears.
-struct FillArgs {
-    void* table;
-    unsigned long long row_bytes, stride_bytes;
-    unsigned rows;
-    int flat;              // rows follow each other without gaps, from a 16-byte boundary
-};
-
-__device__ __forceinline__ void clear_table(const FillArgs& f, unsigned part, unsigned parts) {
-    if (f.flat) {
-        const unsigned long long bytes = f.row_bytes * f.rows, pieces = bytes / 16;
-        uint4* p = (uint4*)f.table;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        for (unsigned long long i = (unsigned long long)part * blockDim.x + threadIdx.x; i < pieces;
-             i += (unsigned long long)parts * blockDim.x)
-            p[i] = zero;
-        if (part == 0)
-            for (unsigned long long i = pieces * 16 + threadIdx.x * 2; i < bytes; i += blockDim.x * 2)
-                *(unsigned short*)((char*)f.table + i) = 0;
-    } else {
-        const unsigned wave = part * (blockDim.x >> 6) + (threadIdx.x >> 6), waves = parts * (blockDim.x >> 6);
-        for (unsigned r = wave; r < f.rows; r += waves) {
-            unsigned short* row = (unsigned short*)((char*)f.table + (unsigned long long)r * f.stride_bytes);
-            for (unsigned long long i = threadIdx.x & 63; i < f.row_bytes / 2; i += 64) row[i] = 0;
+// All pairs within chunks of kChunk places: a workgroup ranks 64 places, one a lane; its wavefronts share
+// the places of the chunk they are compared with, which lie in LDS as keys.  Equal keys rank in order of
+// their places.  Two to three instructions a pair: 2 us for a chunk, whatever the number of chunks.
+__global__ __launch_bounds__(kSortThreads) void rank_chunk_kernel(SortArgs a) {
+    __shared__ uint4 keys4[kChunk / 4];
+    unsigned* keys = reinterpret_cast<unsigned*>(keys4);
+    const unsigned first = blockIdx.x * 64 / kChunk * kChunk;        // of the chunk
+    for (unsigned i = threadIdx.x; i < kChunk; i += kSortThreads)
+        keys[i] = first + i < a.n ? key_of(a.tokens[first + i], a.vocab, a.pad) : ~0u;
+    __syncthreads();
+    const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned base = blockIdx.x * 64 - first, mine = keys[base + lane];
+    constexpr unsigned kEach = kChunk / kSortWaves;
+    unsigned count = 0;
+    for (unsigned c = wave * kEach; c < (wave + 1) * kEach; c += 64) {
+        const uint4* k4 = keys4 + c / 4;
+        if (c < base) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const uint4 k = k4[j];
+                count += (k.x <= mine) + (k.y <= mine) + (k.z <= mine) + (k.w <= mine);
+            }
+        } else if (c > base) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const uint4 k = k4[j];
+                count += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {                  // (keys are below 2^32 - 1: an equal one in front counts)
+                const uint4 k = k4[j];
+                count += (k.x < mine + (4 * j < lane)) + (k.y < mine + (4 * j + 1 < lane)) + (k.z < mine + (4 * j + 2 < lane)) +
+                         (k.w < mine + (4 * j + 3 < lane));
+            }
         }
     }
+    __syncthreads();
+    keys[wave * 64 + lane] = count;
+    __syncthreads();
+    if (wave != 0 || first + base + lane >= a.n) return;
+    unsigned rank = 0;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) rank += keys[w * 64 + lane];
+    a.key_out[first + rank] = mine;
+    a.place_out[first + rank] = first + base + lane;
 }
 
-// All places in one workgroup (n <= kOneSortMax); the others of the grid clear the table.
-__global__ __launch_bounds__(kSortThreads) void sort_one_kernel(SortArgs a, FillArgs f, int total_bits) {
-    __shared__ unsigned keys[kOneSortMax];
-    __shared__ unsigned short places[kOneSortMax];
-    __shared__ unsigned hist[kSortWaves << kOneDigitBits];
-    __shared__ unsigned sh[kSortWaves];
-    if (blockIdx.x > 0) {
-        clear_table(f, blockIdx.x - 1, gridDim.x - 1);
-        return;
-    }
-    const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    // wavefront w owns items [w * per, (w + 1) * per) of the list in its present order
-    const unsigned rounds = (a.n + kSortThreads - 1) / kSortThreads;      // 64-item rounds a wavefront
-    const unsigned base = wave * rounds * 64;
-    unsigned key[kItems], place[kItems], rank[kItems];
+// The rank among all chunks: a place's rank in its own, and in every other chunk the number of keys below
+// it (chunks behind) or not above it (chunks in front), found by halving in all chunks at once.
+__global__ __launch_bounds__(kEmbBlock) void rank_join_kernel(SortArgs a) {
+    __shared__ unsigned keys[kRankMax];
+    constexpr int kChunks = kRankMax / kChunk;
+    const unsigned i = blockIdx.x * kEmbBlock + threadIdx.x;
+    const unsigned place = i < a.n ? a.place_in[i] : 0u;
+    const unsigned whole = a.n / 4;
+    for (unsigned k = threadIdx.x; k < whole; k += kEmbBlock)
+        reinterpret_cast<uint4*>(keys)[k] = reinterpret_cast<const uint4*>(a.key_in)[k];
+    for (unsigned k = whole * 4 + threadIdx.x; k < kRankMax; k += kEmbBlock) keys[k] = k < a.n ? a.key_in[k] : ~0u;
+    __syncthreads();
+    if (i >= a.n) return;
+    const unsigned mine = keys[i], own = i / kChunk;
+    unsigned low[kChunks];                                          // keys in front of it are below the limit
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-        const unsigned i = base + k * 64 + lane;
-        const bool in = (unsigned)k < rounds && i < a.n;
-        key[k] = in ? key_of(a.tokens[i], a.vocab, a.pad) : 0u;
-        place[k] = i;
-    }
-    const int passes = (total_bits + kOneDigitBits - 1) / kOneDigitBits;
-    const int bits = (total_bits + passes - 1) / passes;
-    const unsigned digits = 1u << bits;
-    for (int p = 0; p < passes; ++p) {
-        for (unsigned i = threadIdx.x; i < kSortWaves * digits; i += kSortThreads) hist[i] = 0;
-        __syncthreads();
+    for (int c = 0; c < kChunks; ++c) low[c] = 0;
+    // (keys are below 2^31, what lies behind the last is above every limit)
 #pragma unroll
-        for (int k = 0; k < kItems; ++k) {
-            if ((unsigned)k < rounds) {
-                const bool in = base + k * 64 + lane < a.n;
-                const unsigned d = (key[k] >> (p * bits)) & (digits - 1);
-                const unsigned long long m = same_digit(d, bits, in);
-                const unsigned before = __popcll(m & ((1ull << lane) - 1));
-                unsigned* h = hist + wave * digits + d;
-                // (a wavefront's LDS operations are carried out in order: every lane reads the count
-                // before the first lane of its digit raises it)
-                const unsigned seen = in ? *(volatile unsigned*)h : 0u;
-                if (in && before == 0) *(volatile unsigned*)h = seen + __popcll(m);
-                rank[k] = seen + before;
-            }
-        }
-        __syncthreads();
-        // where each wavefront's items of a digit start: digits first, wavefronts within a digit
-        const unsigned e = threadIdx.x;
-        const bool mine = e < kSortWaves * digits;
-        const unsigned w = e % kSortWaves, d = e / kSortWaves;
-        const unsigned start = scan_exclusive(mine ? hist[w * digits + d] : 0u, sh);
-        if (mine) hist[w * digits + d] = start;
-        __syncthreads();
+    for (unsigned step = kChunk / 2; step > 0; step /= 2) {
 #pragma unroll
-        for (int k = 0; k < kItems; ++k) {
-            if ((unsigned)k < rounds && base + k * 64 + lane < a.n) {
-                const unsigned dk = (key[k] >> (p * bits)) & (digits - 1);
-                const unsigned to = hist[wave * digits + dk] + rank[k];
-                keys[to] = key[k];
-                places[to] = (unsigned short)place[k];
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kItems; ++k) {
-            const unsigned i = base + k * 64 + lane;
-            if ((unsigned)k < rounds && i < a.n) {
-                key[k] = keys[i];
-                place[k] = places[i];
-            }
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-        const unsigned i = base + k * 64 + lane;
-        if ((unsigned)k < rounds && i < a.n) {
-            a.key_out[i] = key[k];
-            a.place_out[i] = place[k];
+        for (int c = 0; c < kChunks; ++c) {
+            const unsigned limit = (unsigned)c < own ? mine + 1 : mine;
+            if (keys[c * kChunk + low[c] + step - 1] < limit) low[c] += step;
         }
     }
+    unsigned rank = i - own * kChunk;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        // (kChunk - 1 keys have been told apart: the last one)
+        const unsigned limit = (unsigned)c < own ? mine + 1 : mine;
+        if (keys[c * kChunk + low[c]] < limit) ++low[c];
+        if ((unsigned)c != own) rank += low[c];
+    }
+    a.key_out[rank] = mine;
+    a.place_out[rank] = place;
 }
 
-// Tiles, first launch: the counts of the first digit of every tile, the counters of the second pass
-// cleared; the other workgroups clear the table.
-__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a, FillArgs f) {
+template <bool FIRST>
+__device__ __forceinline__ unsigned tile_key(const SortArgs& a, unsigned i) {
+    if constexpr (FIRST) return key_of(a.tokens[i], a.vocab, a.pad);
+    else return a.key_in[i];
+}
+
+// Tiles: the counts of a pass's digit in every tile.
+template <bool FIRST>
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a) {
     __shared__ unsigned hist[kTileDigits];
-    if (blockIdx.x >= a.tiles) {
-        clear_table(f, blockIdx.x - a.tiles, gridDim.x - a.tiles);
-        return;
-    }
-    for (unsigned i = threadIdx.x; i < kTileDigits; i += kSortThreads) {
-        hist[i] = 0;
-        if (a.next) a.next[blockIdx.x * kTileDigits + i] = 0;
-    }
+    for (unsigned i = threadIdx.x; i < kTileDigits; i += kSortThreads) hist[i] = 0;
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kTileItems; ++k) {
         const unsigned i = blockIdx.x * kTile + k * kSortThreads + threadIdx.x;
-        if (i < a.n) atomicAdd(&hist[(key_of(a.tokens[i], a.vocab, a.pad) >> a.shift) & ((1u << a.bits) - 1)], 1u);
+        if (i < a.n) atomicAdd(&hist[(tile_key<FIRST>(a, i) >> a.shift) & ((1u << a.bits) - 1)], 1u);
     }
     __syncthreads();
     for (unsigned i = threadIdx.x; i < kTileDigits; i += kSortThreads) a.table[blockIdx.x * kTileDigits + i] = hist[i];
 }
 
-// Clears the counters of the pass after the next (three passes or more).
-__global__ __launch_bounds__(kEmbBlock) void sort_clear_kernel(unsigned* p, unsigned n) {
-    const unsigned i = blockIdx.x * kEmbBlock + threadIdx.x;
-    if (i < n) p[i] = 0;
-}
-
 // Tiles, a pass: ranks within the tile, offset by the counts of the tiles before it and of the
-// smaller digits; counts the next digit of every item at the tile it goes to.
+// smaller digits.
 template <bool FIRST>
 __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortArgs a) {
     __shared__ unsigned hist[kSortWaves * kTileDigits];
     __shared__ unsigned start[kTileDigits];
+    __shared__ unsigned part[kTileDigits];
     __shared__ unsigned sh[kSortWaves];
     const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const unsigned digits = 1u << a.bits;
-    for (unsigned i = threadIdx.x; i < kSortWaves * digits; i += kSortThreads) hist[i] = 0;
-    // digit `threadIdx.x`: items of smaller tiles, and of all
-    unsigned before_me = 0, all = 0;
-    if (threadIdx.x < digits)
-        for (unsigned t = 0; t < a.tiles; ++t) {
-            const unsigned c = a.table[t * kTileDigits + threadIdx.x];
-            all += c;
-            if (t < blockIdx.x) before_me += c;
-        }
-    const unsigned smaller = scan_exclusive(threadIdx.x < digits ? all : 0u, sh);      // (ends with a barrier)
-    if (threadIdx.x < digits) start[threadIdx.x] = smaller + before_me;
     unsigned key[kTileItems], place[kTileItems], rank[kTileItems];
     const unsigned base = blockIdx.x * kTile + wave * (kTileItems * 64);
 #pragma unroll
     for (int k = 0; k < kTileItems; ++k) {
         const unsigned i = base + k * 64 + lane;
         const bool in = i < a.n;
-        if constexpr (FIRST) {
-            key[k] = in ? key_of(a.tokens[i], a.vocab, a.pad) : 0u;
-            place[k] = i;
-        } else {
-            key[k] = in ? a.key_in[i] : 0u;
-            place[k] = in ? a.place_in[i] : 0u;
-        }
+        key[k] = in ? tile_key<FIRST>(a, i) : 0u;
+        place[k] = FIRST ? i : in ? a.place_in[i] : 0u;
     }
+    for (unsigned i = threadIdx.x; i < kSortWaves * digits; i += kSortThreads) hist[i] = 0;
+    // a digit's items in smaller tiles, and in all: two lanes share a digit, each taking every other tile,
+    // 16 counts in flight
+    static_assert(kSortThreads == 2 * kTileDigits, "two lanes a digit");
+    const unsigned digit = threadIdx.x & (kTileDigits - 1), half = threadIdx.x / kTileDigits;
+    unsigned before_me = 0, all = 0;
+    if (digit < digits)
+        for (unsigned t0 = half; t0 < a.tiles; t0 += 32) {
+            unsigned c[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) c[k] = t0 + 2 * k < a.tiles ? a.table[(t0 + 2 * k) * kTileDigits + digit] : 0u;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                all += c[k];
+                if (t0 + 2 * k < blockIdx.x) before_me += c[k];
+            }
+        }
+    if (half) start[digit] = all, part[digit] = before_me;
+    __syncthreads();
+    if (!half) {
+        all += start[digit];
+        before_me += part[digit];
+    }
+    const unsigned smaller = scan_exclusive(half ? 0u : all, sh);          // (lanes of the second half lie behind)
+    if (!half) start[digit] = smaller + before_me;
 #pragma unroll
     for (int k = 0; k < kTileItems; ++k) {
         const bool in = base + k * 64 + lane < a.n;
@@ -317,6 +302,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortArgs a) 
         const unsigned long long m = same_digit(d, a.bits, in);
         const unsigned before = __popcll(m & ((1ull << lane) - 1));
         unsigned* h = hist + wave * digits + d;
+        // (a wavefront's LDS operations are carried out in order: every lane reads the count before
+        // the first lane of its digit raises it)
         const unsigned seen = in ? *(volatile unsigned*)h : 0u;
         if (in && before == 0) *(volatile unsigned*)h = seen + __popcll(m);
         rank[k] = seen + before;
@@ -337,7 +324,6 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortArgs a) 
             const unsigned to = hist[wave * digits + ((key[k] >> a.shift) & (digits - 1))] + rank[k];
             a.key_out[to] = key[k];
             a.place_out[to] = place[k];
-            if (a.next) atomicAdd(&a.next[(to / kTile) * kTileDigits + ((key[k] >> a.next_shift) & ((1u << a.next_bits) - 1))], 1u);
         }
     }
 }
@@ -352,6 +338,7 @@ struct SumArgs {
                                // unit, the part of the one that goes on behind it
     long long dy_stride, table_stride, part_stride;
     unsigned n, vocab, width, units, unit;
+    unsigned workers, slab;    // workgroups that add; behind them one for every `slab` rows of the table to clear
     float scale;
     int accumulate;
 };
@@ -371,99 +358,289 @@ __device__ __forceinline__ void finish_row(const SumArgs& a, unsigned token, uns
     store_piece<TOut, VEC, RAGGED>(to, in, v);
 }
 
-constexpr int kSumAhead = 8;       // rows in flight
+// A row's piece as it lies in memory, so that rows in flight take as few registers as bytes.
+template <class T, int VEC, bool RAGGED>
+__device__ __forceinline__ typename VecOf<T, VEC>::type load_raw(const T* p, int count) {
+    typename VecOf<T, VEC>::type v;
+    if (RAGGED ? count == VEC : count > 0) {
+        if constexpr (RAGGED) v = *reinterpret_cast<const typename VecOf<T, VEC>::loose*>(p);
+        else v = *reinterpret_cast<const typename VecOf<T, VEC>::type*>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            v[i] = (T)0.0f;
+            if (RAGGED && i < count) v[i] = p[i];
+        }
+    }
+    return v;
+}
 
-// A wavefront sums one unit over 64 * VEC columns.
-template <class TIn, class TOut, int VEC, bool RAGGED>
+constexpr int kUnitMax = 64;       // places of a unit: a lane holds one
+
+// Writes zeros to the rows of lanes whose `clear` is set; lane l stands for row r0 + l.
+template <class TOut, bool RAGGED>
+__device__ __forceinline__ void clear_rows(const SumArgs& a, unsigned r0, bool clear) {
+    constexpr int kPiece = 16 / sizeof(TOut);
+    unsigned long long rows = __ballot(clear);
+    const unsigned lane = threadIdx.x & 63, chunks = (a.width + kPiece - 1) / kPiece;
+    float zero[kPiece];
+#pragma unroll
+    for (int j = 0; j < kPiece; ++j) zero[j] = 0.0f;
+    while (rows) {
+        const unsigned r = r0 + __builtin_ctzll(rows);
+        rows &= rows - 1;
+        TOut* row = (TOut*)a.table + (long long)r * a.table_stride;
+        for (unsigned c = lane; c < chunks; c += 64)
+            store_piece<TOut, kPiece, RAGGED>(row + (size_t)c * kPiece, piece_count<kPiece, RAGGED>(c * kPiece, a.width), zero);
+    }
+}
+
+// A wavefront clears those of up to 64 rows that the sorted list does not hold: a lane looks one up.
+template <class TOut, bool RAGGED>
+__device__ __forceinline__ void clear_missing(const SumArgs& a, unsigned r0, unsigned count) {
+    const unsigned lane = threadIdx.x & 63, row = r0 + lane;
+    unsigned low = 0, high = a.n;                          // the first key not below `row` is in [low, high]
+    while (low < high) {
+        const unsigned mid = (low + high) / 2;
+        if (a.keys[mid] < row) low = mid + 1; else high = mid;
+    }
+    const bool holds = low < a.n && a.keys[low] == row;
+    clear_rows<TOut, RAGGED>(a, r0, lane < count && !holds);
+}
+
+// A wavefront sums one unit over 64 * VEC columns.  The unit's keys and places are one load a lane; the
+// rows come in batches of AHEAD, the next batch in flight while one is added.  ADD: the sums are added to
+// the table, whose rows are fetched with the batch in which their token ends.
+template <class TIn, class TOut, int VEC, bool RAGGED, bool ADD>
 __global__ __launch_bounds__(kEmbBlock) void embedding_sum_kernel(SumArgs a, unsigned col_blocks) {
+    constexpr int kAhead = ADD ? 4 : 8;
+    typedef typename VecOf<TIn, VEC>::type Raw;
+    typedef typename VecOf<TOut, VEC>::type Old;
+    if (!ADD && blockIdx.x >= a.workers) {
+        const unsigned r0 = ((blockIdx.x - a.workers) * (kEmbBlock / 64) + (threadIdx.x >> 6)) * a.slab;
+        if (r0 < a.vocab) clear_missing<TOut, RAGGED>(a, r0, min(a.slab, a.vocab - r0));
+        return;
+    }
     const unsigned job = blockIdx.x * (kEmbBlock / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned u = job / col_blocks, cb = job - u * col_blocks;
     if (u >= a.units) return;
-    const unsigned col = (cb * 64 + (threadIdx.x & 63)) * VEC;
+    const unsigned lane = threadIdx.x & 63;
+    const unsigned col = (cb * 64 + lane) * VEC;
     const int in = piece_count<VEC, RAGGED>(col, a.width);
-    const bool live = in > 0;
-    const unsigned begin = u * a.unit, end = min(a.n, begin + a.unit);
-    unsigned token = a.keys[begin];
-    if (token >= a.vocab) return;
+    const unsigned begin = u * a.unit, end = min(a.n, begin + a.unit), count = end - begin;
+    const unsigned my_key = lane < count ? a.keys[begin + lane] : a.vocab;
+    const unsigned my_place = lane < count ? a.places[begin + lane] : 0u;
     const unsigned before = begin > 0 ? a.keys[begin - 1] : ~0u;
+    const unsigned after = end < a.n ? a.keys[end] : ~0u;
+    unsigned token = __builtin_amdgcn_readlane(my_key, 0);
+    if (token >= a.vocab) return;
+    // entries of tokens in the table lie in front of the others
+    const unsigned valid = __popcll(__ballot(lane < count && my_key < a.vocab));
+    const TIn* dy = (const TIn*)a.dy + col;
+    TOut* table = (TOut*)a.table + col;
+    float* part = a.parts + (size_t)u * 2 * a.part_stride + col;
     bool from_before = before == token;
     float acc[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
-    const TIn* dy = (const TIn*)a.dy;
-    for (unsigned i = begin; i < end; i += kSumAhead) {
-        float v[kSumAhead][VEC];
-        unsigned key[kSumAhead];
+    auto key_at = [&](unsigned e) { return e < valid ? (unsigned)__builtin_amdgcn_readlane(my_key, e) : e == count ? after : a.vocab; };
+    Raw rows[kAhead], next[kAhead];
+    Old olds[ADD ? kAhead : 1], next_olds[ADD ? kAhead : 1];
+    auto fetch = [&](unsigned i, Raw (&to)[kAhead], Old (&old)[ADD ? kAhead : 1]) {
 #pragma unroll
-        for (int k = 0; k < kSumAhead; ++k) {
-            const bool more = i + k < end;
-            key[k] = more ? a.keys[i + k] : a.vocab;
-            const unsigned place = more ? a.places[i + k] : 0u;
-            if (live && key[k] < a.vocab) {
-                load_piece<TIn, VEC, RAGGED>(dy + (long long)place * a.dy_stride + col, in, v[k]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) v[k][j] = 0.0f;
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < kSumAhead; ++k) {
-            if (i + k < end) {
-                if (key[k] != token) {
-                    if (live && token < a.vocab) {
-                        if (from_before)
-                            store_from_float<float, VEC>(a.parts + (size_t)u * 2 * a.part_stride + col, acc);
-                        else
-                            finish_row<TOut, VEC, RAGGED>(a, token, col, in, acc);
-                    }
-                    from_before = false;
-                    token = key[k];
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) acc[j] = v[k][j];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) acc[j] += v[k][j];
+        for (int k = 0; k < kAhead; ++k) {
+            if (i + k < valid) {
+                const unsigned place = __builtin_amdgcn_readlane(my_place, i + k);
+                to[k] = load_raw<TIn, VEC, RAGGED>(dy + (long long)place * a.dy_stride, in);
+                if constexpr (ADD) {
+                    const unsigned key = key_at(i + k);
+                    if (key != key_at(i + k + 1)) old[k] = load_raw<TOut, VEC, RAGGED>(table + (long long)key * a.table_stride, in);
                 }
             }
         }
+    };
+    fetch(0, rows, olds);
+    for (unsigned i = 0; i < valid; i += kAhead) {
+        fetch(i + kAhead, next, next_olds);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            if (i + k < valid) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) acc[j] += (float)rows[k][j];
+                const unsigned following = key_at(i + k + 1);
+                if (following != token || i + k + 1 == count) {
+                    // the token ends here, or the unit does
+                    if (in > 0) {
+                        if (from_before) {
+                            store_from_float<float, VEC>(part, acc);
+                        } else if (following == token) {
+                            store_from_float<float, VEC>(part + a.part_stride, acc);
+                        } else {
+                            float v[VEC];
+#pragma unroll
+                            for (int j = 0; j < VEC; ++j) {
+                                v[j] = a.scale * acc[j];
+                                if constexpr (ADD) v[j] += (float)olds[k][j];
+                            }
+                            store_piece<TOut, VEC, RAGGED>(table + (long long)token * a.table_stride, in, v);
+                        }
+                    }
+                    from_before = false;
+                    token = following;
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            rows[k] = next[k];
+            if constexpr (ADD) olds[k] = next_olds[k];
+        }
     }
-    if (!live || token >= a.vocab) return;
-    const bool goes_on = end < a.n && a.keys[end] == token;
-    if (from_before)
-        store_from_float<float, VEC>(a.parts + (size_t)u * 2 * a.part_stride + col, acc);
-    else if (goes_on)
-        store_from_float<float, VEC>(a.parts + ((size_t)u * 2 + 1) * a.part_stride + col, acc);
-    else
-        finish_row<TOut, VEC, RAGGED>(a, token, col, in, acc);
 }
 
-// The units in which a token that crosses their end begins: 4 wavefronts share the parts of 64 * VEC
-// columns, each adding a run of them, and meet in LDS in that order.
-template <class TOut, int VEC, bool RAGGED>
-__global__ __launch_bounds__(kEmbBlock) void embedding_merge_kernel(SumArgs a, unsigned col_blocks) {
-    const unsigned u = blockIdx.x / col_blocks, cb = blockIdx.x - u * col_blocks;
-    const unsigned end = (u + 1) * a.unit;               // (the last unit has no workgroup here)
-    const unsigned token = a.keys[end - 1];
-    if (token >= a.vocab || a.keys[end] != token) return;
-    const unsigned begin = u * a.unit;
-    if (a.keys[begin] == token && begin > 0 && a.keys[begin - 1] == token) return;     // began earlier
-    // units after u that begin with the token: the list is sorted
-    unsigned low = u + 1, high = a.units;                // low does, high (or the end) does not
-    while (high - low > 1) {
-        const unsigned mid = (low + high) / 2;
-        if (a.keys[mid * a.unit] == token) low = mid; else high = mid;
+// Few places, no sort.  A wavefront takes a place: it looks through the tokens for the other places of its
+// token and goes on if its own is the first.  Up to kFewAlone rows it adds by itself,
+// more are shared by the workgroup's wavefronts and their sums meet in LDS in order.  col_parts workgroups
+// share the blocks of columns.  Behind these, workgroups clear the rows of a slab whose token does not occur.
+template <class TIn, class TOut, int VEC, bool RAGGED>
+__global__ __launch_bounds__(kFewWaves * 64) void embedding_few_kernel(SumArgs a, const int32_t* tokens, int pad, unsigned col_parts, unsigned col_blocks) {
+    constexpr int kAhead = kFewAlone;
+    typedef typename VecOf<TIn, VEC>::type Raw;
+    __shared__ unsigned keys[kFew];
+    __shared__ unsigned short found[kFewWaves][kFew];
+    __shared__ float sums[kFewWaves][64 * VEC];
+    __shared__ unsigned counts[kFewWaves], token_of[kFewWaves];
+    const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (blockIdx.x >= a.workers) {
+        unsigned char* occurs = reinterpret_cast<unsigned char*>(found);
+        static_assert(sizeof(found) >= kFewRows, "a slab's marks fit");
+        const unsigned r0 = (blockIdx.x - a.workers) * a.slab, r1 = min(a.vocab, r0 + a.slab);
+        for (unsigned r = threadIdx.x; r < r1 - r0; r += kFewWaves * 64) occurs[r] = 0;
+        __syncthreads();
+        for (unsigned i = threadIdx.x; i < a.n; i += kFewWaves * 64) {
+            const unsigned key = key_of(tokens[i], a.vocab, pad);
+            if (key >= r0 && key < r1) occurs[key - r0] = 1;
+        }
+        __syncthreads();
+        const unsigned each = (r1 - r0 + kFewWaves - 1) / kFewWaves, last = min(r1, r0 + (wave + 1) * each);
+        for (unsigned r = r0 + wave * each; r < last; r += 64)
+            clear_rows<TOut, RAGGED>(a, r, r + lane < last && !occurs[r + lane - r0]);
+        return;
     }
-    const unsigned parts = low - u + 1;
-    const unsigned wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (unsigned i = threadIdx.x; i < kFew; i += kFewWaves * 64) keys[i] = i < a.n ? key_of(tokens[i], a.vocab, pad) : ~0u;
+    __syncthreads();
+    const unsigned group = blockIdx.x / col_parts, cp = blockIdx.x - group * col_parts;
+    // (frequent tokens have their first places near the front: a workgroup's places lie far apart)
+    const unsigned mine = group + wave * (a.workers / col_parts);
+    const unsigned token = mine < a.n ? (unsigned)__builtin_amdgcn_readfirstlane(keys[mine]) : ~0u;
+    unsigned count = 0;
+    if (token < a.vocab) {
+        bool first = true;
+        for (unsigned c = 0; c < a.n && first; c += 256) {             // (kFew keys, a multiple of 256)
+            bool same[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) same[k] = keys[c + k * 64 + lane] == token;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const unsigned at = c + k * 64;
+                const unsigned long long m = __ballot(same[k]);
+                if (same[k]) found[wave][count + __popcll(m & ((1ull << lane) - 1))] = (unsigned short)(at + lane);
+                first = first && (mine >= at + 64 ? m == 0 : mine < at || (m & ((1ull << (mine - at)) - 1)) == 0);
+                count += __popcll(m);
+            }
+        }
+        if (!first) count = 0;
+    }
+    if (lane == 0) {
+        counts[wave] = count;
+        token_of[wave] = token;
+    }
+    __syncthreads();
+    // the sum of entries [e0, e1) of the list of wavefront w
+    auto add = [&](unsigned w, unsigned e0, unsigned e1, unsigned col, int in, float (&acc)[VEC]) {
+        const TIn* dy = (const TIn*)a.dy + col;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
+        for (unsigned e = e0; e < e1; e += kAhead) {
+            Raw rows[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                if (e + k < e1) {
+                    const unsigned place = __builtin_amdgcn_readfirstlane((unsigned)found[w][e + k]);
+                    rows[k] = load_raw<TIn, VEC, RAGGED>(dy + (long long)place * a.dy_stride, in);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                if (e + k < e1) {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) acc[j] += (float)rows[k][j];
+                }
+            }
+        }
+    };
+    for (unsigned cb = cp; cb < col_blocks; cb += col_parts) {
+        const unsigned col = (cb * 64 + lane) * VEC;
+        const int in = piece_count<VEC, RAGGED>(col, a.width);
+        float acc[VEC];
+        if (count > 0 && count <= kFewAlone) {
+            add(wave, 0, count, col, in, acc);
+            if (in > 0) finish_row<TOut, VEC, RAGGED>(a, token, col, in, acc);
+        }
+        for (unsigned w = 0; w < kFewWaves; ++w) {
+            const unsigned many = counts[w];
+            if (many <= kFewAlone) continue;
+            const unsigned share = (many + kFewWaves - 1) / kFewWaves;
+            add(w, min(many, wave * share), min(many, (wave + 1) * share), col, in, acc);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) sums[wave][j * 64 + lane] = acc[j];
+            __syncthreads();
+            if (wave == w && in > 0) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    acc[j] = sums[0][j * 64 + lane];
+#pragma unroll
+                    for (int v = 1; v < kFewWaves; ++v) acc[j] += sums[v][j * 64 + lane];
+                }
+                finish_row<TOut, VEC, RAGGED>(a, token_of[w], col, in, acc);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// The units in which a token that crosses their end begins: the wavefronts of a workgroup share the parts of
+// 64 * VEC columns, each adding a run of them, and meet in LDS in that order.
+constexpr int kMergeWaves = 8;
+
+template <class TOut, int VEC, bool RAGGED>
+__global__ __launch_bounds__(kMergeWaves * 64) void embedding_merge_kernel(SumArgs a, unsigned col_blocks) {
+    const unsigned u = blockIdx.x / col_blocks, cb = blockIdx.x - u * col_blocks;
+    const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const unsigned begin = u * a.unit, end = begin + a.unit;               // (the last unit has no workgroup here)
+    // lane l looks at the first key of unit u + 1 + l: the units behind u that begin with its last token
+    const unsigned token = a.keys[end - 1];
+    const unsigned here = a.keys[begin], before = begin > 0 ? a.keys[begin - 1] : ~0u;
+    unsigned more = 0;
+    for (unsigned v = u + 1; v < a.units; v += 64) {
+        const bool same = v + lane < a.units && a.keys[(v + lane) * a.unit] == token;
+        const unsigned long long m = __ballot(same);
+        const unsigned run = ~m ? __builtin_ctzll(~m) : 64;
+        more += run;
+        if (run < 64) break;
+    }
+    if (token >= a.vocab || more == 0 || (here == token && before == token)) return;   // (the last: began earlier)
+    const unsigned parts = more + 1;
     const unsigned col = (cb * 64 + lane) * VEC;
     const int in = piece_count<VEC, RAGGED>(col, a.width);
-    const bool live = in > 0;
-    const unsigned share = (parts + 3) / 4;
+    const unsigned share = (parts + kMergeWaves - 1) / kMergeWaves;
     const unsigned p0 = min(parts, wave * share), p1 = min(parts, p0 + share);
     float acc[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
-    if (live)
+    if (in > 0)
         for (unsigned p = p0; p < p1; p += 4) {
             float v[4][VEC];
 #pragma unroll
@@ -482,14 +659,16 @@ __global__ __launch_bounds__(kEmbBlock) void embedding_merge_kernel(SumArgs a, u
                 for (int i = 0; i < VEC; ++i) acc[i] += v[k][i];
             }
         }
-    __shared__ float sh[4][64 * VEC];
+    __shared__ float sh[kMergeWaves][64 * VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) sh[wave][i * 64 + lane] = acc[i];
     __syncthreads();
-    if (wave != 0 || !live) return;
+    if (wave != 0 || in <= 0) return;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i)
-        acc[i] = (sh[0][i * 64 + lane] + sh[1][i * 64 + lane]) + (sh[2][i * 64 + lane] + sh[3][i * 64 + lane]);
+    for (int i = 0; i < VEC; ++i) {
+#pragma unroll
+        for (int w = 1; w < kMergeWaves; ++w) acc[i] += sh[w][i * 64 + lane];
+    }
     finish_row<TOut, VEC, RAGGED>(a, token, col, in, acc);
 }
 
@@ -565,7 +744,8 @@ int launch_lookup(const ContextView& c, const ngh_embedding_spec* s) {
 // How the gradient of n places is worked on, and where its parts lie in the workspace.
 struct GradPlan {
     int bits, passes;          // of the key, tiles only
-    unsigned tiles;            // 0: one workgroup sorts
+    bool few;                  // no sort
+    unsigned tiles;            // 0: ranked in chunks
     unsigned unit, units, col_blocks;
     bool ragged;
     size_t part_stride;
@@ -573,51 +753,80 @@ struct GradPlan {
 };
 
 GradPlan plan_grad(const ngh_embedding_spec* s, int cus) {
-    GradPlan g;
+    GradPlan g{};
     const unsigned n = (unsigned)s->rows;
     g.bits = 1;
     while ((1ull << g.bits) <= (unsigned long long)s->vocab) ++g.bits;           // keys 0 .. vocab
-    g.tiles = n <= (unsigned)kOneSortMax ? 0 : (n + kTile - 1) / kTile;
+    g.few = n <= (unsigned)kFew;
+    g.tiles = n <= (unsigned)kRankMax ? 0 : (n + kTile - 1) / kTile;
     g.passes = (g.bits + kTileDigitBits - 1) / kTileDigitBits;
     const int vec = size_of(s->y_dtype) == 2 ? 8 : 4;
     g.ragged = !whole_pieces(s, vec);
     g.col_blocks = (unsigned)((s->width + 64 * vec - 1) / (64 * vec));
     // Units of 64 places while that gives every compute unit 8 wavefronts, shorter ones (down to 8)
     // for fewer: a unit's parts cost two fp32 rows where its tokens cross its ends.
-    g.unit = 64;
+    g.unit = kUnitMax;
     while (g.unit > 8 && (unsigned long long)((n + g.unit - 1) / g.unit) * g.col_blocks < 8ull * cus) g.unit /= 2;
     g.units = (n + g.unit - 1) / g.unit;
     g.part_stride = ((size_t)s->width + 7) / 8 * 8;
     auto room = [](size_t b) { return (b + 255) / 256 * 256; };
     size_t at = 0;
-    g.keys_a = at, at += room(4ull * n);
-    g.places_a = at, at += room(4ull * n);
-    g.keys_b = at, at += g.tiles ? room(4ull * n) : 0;
-    g.places_b = at, at += g.tiles ? room(4ull * n) : 0;
-    g.tables = at, at += (size_t)g.tiles * 3 * kTileDigits * 4;
-    g.parts = at, at += g.units > 1 ? (size_t)g.units * 2 * g.part_stride * 4 : 0;
+    if (!g.few) {
+        g.keys_a = at, at += room(4ull * n);
+        g.places_a = at, at += room(4ull * n);
+        g.keys_b = at, at += room(4ull * n);
+        g.places_b = at, at += room(4ull * n);
+        g.tables = at, at += (size_t)g.tiles * kTileDigits * 4;
+        g.parts = at, at += g.units > 1 ? (size_t)g.units * 2 * g.part_stride * 4 : 0;
+    }
     g.bytes = at;
     return g;
 }
 
+// Workgroups that clear the table, a.slab rows for each of `parts` parts of one: about `wgs` of them.
+unsigned slabs_of(SumArgs& a, unsigned wgs, unsigned most, unsigned parts) {
+    if (a.accumulate || a.vocab == 0) return 0;
+    a.slab = std::min(most, std::max(1u, (a.vocab + wgs * parts - 1) / (wgs * parts)));
+    const unsigned per = a.slab * parts;
+    return (a.vocab + per - 1) / per;
+}
+
 template <class TIn, class TOut, bool RAGGED>
-int launch_sums(const ContextView& c, const SumArgs& a, unsigned col_blocks) {
+int launch_sums(const ContextView& c, SumArgs a, unsigned col_blocks) {
     constexpr int kVec = 16 / sizeof(TIn);
     const unsigned long long jobs = (unsigned long long)a.units * col_blocks;
     if (jobs >= (1ull << 31)) return report(NGH_E_UNSUPPORTED, "ngh_embedding_grad: grid too large");
-    hipLaunchKernelGGL((embedding_sum_kernel<TIn, TOut, kVec, RAGGED>), dim3((unsigned)((jobs + 3) / 4)), dim3(kEmbBlock), 0, c.stream, a,
-                       col_blocks);
+    a.workers = (unsigned)((jobs + 3) / 4);
+    const unsigned grid = a.workers + slabs_of(a, 4 * c.cus, 64, kEmbBlock / 64);
+    if (a.accumulate) hipLaunchKernelGGL((embedding_sum_kernel<TIn, TOut, kVec, RAGGED, true>), dim3(grid), dim3(kEmbBlock), 0, c.stream, a, col_blocks);
+    else hipLaunchKernelGGL((embedding_sum_kernel<TIn, TOut, kVec, RAGGED, false>), dim3(grid), dim3(kEmbBlock), 0, c.stream, a, col_blocks);
     NGH_HIP_TRY(hipGetLastError());
     if (a.units > 1) {
-        hipLaunchKernelGGL((embedding_merge_kernel<TOut, kVec, RAGGED>), dim3((a.units - 1) * col_blocks), dim3(kEmbBlock), 0, c.stream, a,
+        hipLaunchKernelGGL((embedding_merge_kernel<TOut, kVec, RAGGED>), dim3((a.units - 1) * col_blocks), dim3(kMergeWaves * 64), 0, c.stream, a,
                            col_blocks);
         NGH_HIP_TRY(hipGetLastError());
     }
     return NGH_OK;
 }
 
+template <class TIn, class TOut, bool RAGGED>
+int launch_few(const ContextView& c, SumArgs a, const ngh_embedding_spec* s, unsigned col_blocks) {
+    constexpr int kVec = 16 / sizeof(TIn);
+    // the columns are dealt out while that gives every compute unit no more than four workgroups
+    const unsigned groups = (a.n + kFewWaves - 1) / kFewWaves;
+    const unsigned col_parts = std::min(col_blocks, std::max(1u, 4u * c.cus / std::max(1u, groups)));
+    a.workers = groups * col_parts;
+    const unsigned grid = a.workers + slabs_of(a, 2 * c.cus, kFewRows, 1);
+    if (!grid) return NGH_OK;
+    hipLaunchKernelGGL((embedding_few_kernel<TIn, TOut, kVec, RAGGED>), dim3(grid), dim3(kFewWaves * 64), 0, c.stream, a, s->tokens, (int)s->pad_idx,
+                       col_parts, col_blocks);
+    NGH_HIP_TRY(hipGetLastError());
+    return NGH_OK;
+}
+
 template <class TIn, class TOut>
-int launch_sums(const ContextView& c, const SumArgs& a, const GradPlan& g) {
+int launch_sums(const ContextView& c, const SumArgs& a, const ngh_embedding_spec* s, const GradPlan& g) {
+    if (g.few) return g.ragged ? launch_few<TIn, TOut, true>(c, a, s, g.col_blocks) : launch_few<TIn, TOut, false>(c, a, s, g.col_blocks);
     return g.ragged ? launch_sums<TIn, TOut, true>(c, a, g.col_blocks) : launch_sums<TIn, TOut, false>(c, a, g.col_blocks);
 }
 
@@ -680,67 +889,46 @@ int ngh_embedding_grad(ngh_context* ctx, const ngh_embedding_spec* spec) {
     DeviceScope scope(c.device);
     if (!scope.ok()) return report(NGH_E_RUNTIME, "ngh_embedding_grad: the context's device cannot be made current");
 
-    FillArgs f;
-    f.table = spec->table;
-    f.row_bytes = (unsigned long long)spec->width * te;
-    f.stride_bytes = (unsigned long long)spec->table_stride * te;
-    f.rows = (unsigned)spec->vocab;
-    f.flat = (spec->table_stride == spec->width || spec->vocab == 1) && (uintptr_t)spec->table % 16 == 0;
-    unsigned fill_wgs = 0;
-    if (!spec->accumulate) {
-        // 64 KiB a workgroup at least, two workgroups a compute unit at most
-        const unsigned long long bytes = f.row_bytes * f.rows;
-        fill_wgs = (unsigned)std::max<unsigned long long>(1, std::min<unsigned long long>((bytes + 65535) / 65536, 2ull * c.cus));
-    }
     char* ws = (char*)spec->workspace;
-    SortArgs s;
+    SortArgs s{};
     s.tokens = spec->tokens;
     s.n = (unsigned)spec->rows;
     s.vocab = (unsigned)spec->vocab;
     s.pad = spec->pad_idx;
-    s.key_in = s.place_in = nullptr;
-    s.key_out = (unsigned*)(ws + g.keys_a);
-    s.place_out = (unsigned*)(ws + g.places_a);
-    s.table = s.next = nullptr;
     s.tiles = g.tiles;
-    s.shift = s.bits = s.next_shift = s.next_bits = 0;
-    if (g.tiles == 0) {
-        hipLaunchKernelGGL(sort_one_kernel, dim3(1 + fill_wgs), dim3(kSortThreads), 0, c.stream, s, f, g.bits);
+    s.table = (unsigned*)(ws + g.tables);
+    if (!g.few && g.tiles == 0) {
+        s.key_out = (unsigned*)(ws + g.keys_b);
+        s.place_out = (unsigned*)(ws + g.places_b);
+        hipLaunchKernelGGL(rank_chunk_kernel, dim3((s.n + 63) / 64), dim3(kSortThreads), 0, c.stream, s);
         NGH_HIP_TRY(hipGetLastError());
-    } else {
-        unsigned* tables[3];
-        for (int i = 0; i < 3; ++i) tables[i] = (unsigned*)(ws + g.tables) + (size_t)i * g.tiles * kTileDigits;
+        s.key_in = s.key_out;
+        s.place_in = s.place_out;
+        s.key_out = (unsigned*)(ws + g.keys_a);
+        s.place_out = (unsigned*)(ws + g.places_a);
+        hipLaunchKernelGGL(rank_join_kernel, dim3((s.n + kEmbBlock - 1) / kEmbBlock), dim3(kEmbBlock), 0, c.stream, s);
+        NGH_HIP_TRY(hipGetLastError());
+    } else if (!g.few) {
         const int digit = (g.bits + g.passes - 1) / g.passes;
         for (int p = 0; p < g.passes; ++p) {
-            const bool last = p + 1 == g.passes;
             s.shift = p * digit;
             s.bits = std::min(digit, g.bits - s.shift);
-            s.next_shift = s.shift + s.bits;
-            s.next_bits = last ? 0 : std::min(digit, g.bits - s.next_shift);
-            s.table = tables[p % 3];
-            s.next = last ? nullptr : tables[(p + 1) % 3];
             const bool a_out = (g.passes - 1 - p) % 2 == 0;            // the last pass ends in the first pair
             s.key_out = (unsigned*)(ws + (a_out ? g.keys_a : g.keys_b));
             s.place_out = (unsigned*)(ws + (a_out ? g.places_a : g.places_b));
-            s.key_in = (unsigned*)(ws + (a_out ? g.keys_b : g.keys_a));
-            s.place_in = (unsigned*)(ws + (a_out ? g.places_b : g.places_a));
+            s.key_in = (const unsigned*)(ws + (a_out ? g.keys_b : g.keys_a));
+            s.place_in = (const unsigned*)(ws + (a_out ? g.places_b : g.places_a));
             if (p == 0) {
-                hipLaunchKernelGGL(sort_count_kernel, dim3(g.tiles + fill_wgs), dim3(kSortThreads), 0, c.stream, s, f);
-                NGH_HIP_TRY(hipGetLastError());
+                hipLaunchKernelGGL(sort_count_kernel<true>, dim3(g.tiles), dim3(kSortThreads), 0, c.stream, s);
                 hipLaunchKernelGGL(sort_scatter_kernel<true>, dim3(g.tiles), dim3(kSortThreads), 0, c.stream, s);
             } else {
-                if (!last) {
-                    const unsigned words = g.tiles * kTileDigits;
-                    hipLaunchKernelGGL(sort_clear_kernel, dim3((words + kEmbBlock - 1) / kEmbBlock), dim3(kEmbBlock), 0, c.stream, s.next, words);
-                    NGH_HIP_TRY(hipGetLastError());
-                }
+                hipLaunchKernelGGL(sort_count_kernel<false>, dim3(g.tiles), dim3(kSortThreads), 0, c.stream, s);
                 hipLaunchKernelGGL(sort_scatter_kernel<false>, dim3(g.tiles), dim3(kSortThreads), 0, c.stream, s);
             }
             NGH_HIP_TRY(hipGetLastError());
         }
     }
-    if (spec->rows == 0) return NGH_OK;
-    SumArgs a;
+    SumArgs a{};
     a.keys = (const unsigned*)(ws + g.keys_a);
     a.places = (const unsigned*)(ws + g.places_a);
     a.dy = spec->y;
@@ -757,11 +945,11 @@ int ngh_embedding_grad(ngh_context* ctx, const ngh_embedding_spec* spec) {
     a.scale = spec->scale;
     a.accumulate = spec->accumulate;
     switch (spec->y_dtype * 16 + spec->table_dtype) {
-        case NGH_F32 * 16 + NGH_F32: return launch_sums<float, float>(c, a, g);
-        case NGH_BF16 * 16 + NGH_F32: return launch_sums<bf16_t, float>(c, a, g);
-        case NGH_F16 * 16 + NGH_F32: return launch_sums<f16_t, float>(c, a, g);
-        case NGH_BF16 * 16 + NGH_BF16: return launch_sums<bf16_t, bf16_t>(c, a, g);
-        default: return launch_sums<f16_t, f16_t>(c, a, g);
+        case NGH_F32 * 16 + NGH_F32: return launch_sums<float, float>(c, a, spec, g);
+        case NGH_BF16 * 16 + NGH_F32: return launch_sums<bf16_t, float>(c, a, spec, g);
+        case NGH_F16 * 16 + NGH_F32: return launch_sums<f16_t, float>(c, a, spec, g);
+        case NGH_BF16 * 16 + NGH_BF16: return launch_sums<bf16_t, bf16_t>(c, a, spec, g);
+        default: return launch_sums<f16_t, f16_t>(c, a, spec, g);
     }
 }
 
