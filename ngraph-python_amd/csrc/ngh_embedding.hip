@@ -37,7 +37,7 @@ constexpr int kFew = 2048;                               // places that need no 
 constexpr int kFewWaves = 8;
 constexpr int kFewAlone = 16;                            // rows a wavefront adds by itself (one batch in flight)
 constexpr int kFewRows = 4096;                           // rows of the table one workgroup clears at most
-constexpr int kTileItems = 4;
+constexpr int kTileItems = 2;
 constexpr int kTile = kSortThreads * kTileItems;
 constexpr int kTileDigitBits = 9;
 constexpr int kTileDigits = 1 << kTileDigitBits;
@@ -611,15 +611,18 @@ __global__ __launch_bounds__(kFewWaves * 64) void embedding_few_kernel(SumArgs a
     }
 }
 
-// The units in which a token that crosses their end begins: the wavefronts of a workgroup share the parts of
-// 64 * VEC columns, each adding a run of them, and meet in LDS in that order.
-constexpr int kMergeWaves = 8;
+// A workgroup for each unit but the last and each block of columns: if a token begins in the unit and goes on
+// behind it, its parts are added in order, up to kMergeAlone by one wavefront, more in shares that meet
+// in LDS.  (A workgroup for all columns of a unit took half as long again: the most frequent token's
+// parts are what the launch waits for.)
+constexpr int kMergeWaves = 4;
+constexpr int kMergeAlone = 8;
 
 template <class TOut, int VEC, bool RAGGED>
 __global__ __launch_bounds__(kMergeWaves * 64) void embedding_merge_kernel(SumArgs a, unsigned col_blocks) {
     const unsigned u = blockIdx.x / col_blocks, cb = blockIdx.x - u * col_blocks;
     const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const unsigned begin = u * a.unit, end = begin + a.unit;               // (the last unit has no workgroup here)
+    const unsigned begin = u * a.unit, end = begin + a.unit;
     // lane l looks at the first key of unit u + 1 + l: the units behind u that begin with its last token
     const unsigned token = a.keys[end - 1];
     const unsigned here = a.keys[begin], before = begin > 0 ? a.keys[begin - 1] : ~0u;
@@ -633,43 +636,48 @@ __global__ __launch_bounds__(kMergeWaves * 64) void embedding_merge_kernel(SumAr
     }
     if (token >= a.vocab || more == 0 || (here == token && before == token)) return;   // (the last: began earlier)
     const unsigned parts = more + 1;
-    const unsigned col = (cb * 64 + lane) * VEC;
-    const int in = piece_count<VEC, RAGGED>(col, a.width);
-    const unsigned share = (parts + kMergeWaves - 1) / kMergeWaves;
-    const unsigned p0 = min(parts, wave * share), p1 = min(parts, p0 + share);
-    float acc[VEC];
+    // the sum of parts [p0, p1) in a block of columns; part 0 is what unit u passed on
+    auto add = [&](unsigned p0, unsigned p1, unsigned col, int in, float (&acc)[VEC]) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
-    if (in > 0)
-        for (unsigned p = p0; p < p1; p += 4) {
-            float v[4][VEC];
+        for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
+        if (in <= 0) return;
+        for (unsigned p = p0; p < p1; p += kMergeAlone) {
+            float v[kMergeAlone][VEC];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < kMergeAlone; ++k) {
+                if (p + k < p1)
+                    load_as_float<float, VEC>(a.parts + ((size_t)(u + p + k) * 2 + (p + k == 0 ? 1 : 0)) * a.part_stride + col, v[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < kMergeAlone; ++k) {
                 if (p + k < p1) {
-                    const unsigned q = u + p + k;         // part 0 is what unit u passed on
-                    load_as_float<float, VEC>(a.parts + ((size_t)q * 2 + (p + k == 0 ? 1 : 0)) * a.part_stride + col, v[k]);
-                } else {
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) v[k][i] = 0.0f;
+                    for (int i = 0; i < VEC; ++i) acc[i] += v[k][i];
                 }
             }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) acc[i] += v[k][i];
-            }
         }
-    __shared__ float sh[kMergeWaves][64 * VEC];
+    };
+    float acc[VEC];
+    const unsigned col = (cb * 64 + lane) * VEC;
+    const int in = piece_count<VEC, RAGGED>(col, a.width);
+    if (parts <= kMergeAlone) {
+        if (wave != 0) return;
+        add(0, parts, col, in, acc);
+    } else {
+        __shared__ float sh[kMergeWaves][64 * VEC];
+        const unsigned share = (parts + kMergeWaves - 1) / kMergeWaves;
+        add(min(parts, wave * share), min(parts, (wave + 1) * share), col, in, acc);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sh[wave][i * 64 + lane] = acc[i];
-    __syncthreads();
-    if (wave != 0 || in <= 0) return;
+        for (int i = 0; i < VEC; ++i) sh[wave][i * 64 + lane] = acc[i];
+        __syncthreads();
+        if (wave != 0) return;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
+        for (int i = 0; i < VEC; ++i) {
 #pragma unroll
-        for (int w = 1; w < kMergeWaves; ++w) acc[i] += sh[w][i * 64 + lane];
+            for (int w = 1; w < kMergeWaves; ++w) acc[i] += sh[w][i * 64 + lane];
+        }
     }
-    finish_row<TOut, VEC, RAGGED>(a, token, col, in, acc);
+    if (in > 0) finish_row<TOut, VEC, RAGGED>(a, token, col, in, acc);
 }
 
 // ---- host ------------------------------------------------------------------------------------
@@ -797,7 +805,7 @@ int launch_sums(const ContextView& c, SumArgs a, unsigned col_blocks) {
     const unsigned long long jobs = (unsigned long long)a.units * col_blocks;
     if (jobs >= (1ull << 31)) return report(NGH_E_UNSUPPORTED, "ngh_embedding_grad: grid too large");
     a.workers = (unsigned)((jobs + 3) / 4);
-    const unsigned grid = a.workers + slabs_of(a, 4 * c.cus, 64, kEmbBlock / 64);
+    const unsigned grid = a.workers + slabs_of(a, 16 * c.cus, 64, kEmbBlock / 64);
     if (a.accumulate) hipLaunchKernelGGL((embedding_sum_kernel<TIn, TOut, kVec, RAGGED, true>), dim3(grid), dim3(kEmbBlock), 0, c.stream, a, col_blocks);
     else hipLaunchKernelGGL((embedding_sum_kernel<TIn, TOut, kVec, RAGGED, false>), dim3(grid), dim3(kEmbBlock), 0, c.stream, a, col_blocks);
     NGH_HIP_TRY(hipGetLastError());
