@@ -4,16 +4,20 @@
 // and backward, with T the transpose of N's Jacobian, T(t; x) = r (t - xh mean(t xh) [- mean(t)]):
 //     d = dh + T(dy w; h);   dx = alpha d;   dg += d u;   e = d g;   dp += e bh;   dq += e;
 //     db = T(e p; b);   dw += dy hh;   dz += dy
-// A row is held in registers as fp32 from its one load on (C chunks of VEC elements a lane, a row on
-// NW wavefronts or, NW = 1, on a power of two of lanes), so the forward pass reads x and b and writes
-// h and y once, the backward pass reads dh, dy, h and b and writes dx and db: both are bound by
-// memory.  The variance of the layer norm is taken around the mean, in registers.  The statistics are
+// A row is held in registers from its one load on (C pieces of VEC elements a lane, a row on as many
+// wavefronts as it fills or, not SEVERAL, on a power of two of lanes), so the forward pass reads x and
+// b and writes h and y once, the backward pass reads dh, dy, h and b and writes dx and db: both are
+// bound by memory.  The variance of the layer norm is taken around the mean, in registers.  The statistics are
 // computed again in the backward pass: a reduction that is there anyway, and no operand.
 #pragma once
 #include <hip/hip_runtime.h>
 
 #include "ngh_internal.h"
 #include "ngh_rows.h"
+
+// Products and sums contract to fused multiply-adds here: one rounding less each, and the backward kernel is
+// as near to its vector instructions as to memory.
+#pragma clang fp contract(fast)
 
 namespace ngh {
 
@@ -23,13 +27,15 @@ struct NormArgs {
     float* parts;                  // backward: [part][vector][part_stride] sums of a part's rows
     long long x_stride, b_stride, gate_stride, h_stride, y_stride, dy_stride, dh_stride, dx_stride, db_stride, dgate_stride, part_stride;
     unsigned rows, width, gate_rows;
-    int lanes;                     // NW == 1: lanes along a row
-    int layer, post, param_f32;
-    float eps, alpha, inv_width;
+    int lanes;                     // along a row: whole wavefronts, or a power of two up to 64
+    int post, param_f32;
+    float eps, alpha, inv_width, width_f;      // (a mean is a quotient: a row of equal elements is all zeros behind it)
     // backward: rows [part * per_part, ...) of a span of consecutive rows of one gate row, or several whole ones
     unsigned span_rows, parts_per_span, per_part;
     int vectors;                   // sums a part writes: gain, bias, post gain, post bias, gate (bits), in this order
     int gate_whole;                // a part holds whole gate rows and writes their gradients itself
+    int in_lds;                    // vectors that the workgroup keeps in LDS (bits, kVec*)
+    unsigned lds_stride;           // floats from one of them to the next
 };
 
 constexpr int kVecGain = 1, kVecBias = 2, kVecPostGain = 4, kVecPostBias = 8, kVecGate = 16;
@@ -41,22 +47,23 @@ __device__ __forceinline__ void load_param(const void* p, long long at, int coun
 #pragma unroll
         for (int i = 0; i < VEC; ++i) out[i] = other;
     } else if (f32) {
-        load_piece<float, VEC, RAGGED>((const float*)p + at, count, out);
+        load_piece<float, VEC, RAGGED>((const float*)p + at, count, false, out);
     } else {
-        load_piece<T, VEC, RAGGED>((const T*)p + at, count, out);
+        load_piece<T, VEC, RAGGED>((const T*)p + at, count, false, out);
     }
 }
 
-template <class T, int VEC, int C, int NW, bool RAGGED>
-__global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_norm_kernel(NormArgs a) {
-    constexpr int kThreads = NW == 1 ? 256 : NW * 64;
-    __shared__ float sh[NW == 1 ? 1 : 2 * kRowSumsMax * NW];
+template <class T, int VEC, int C, int THREADS, bool SEVERAL, bool RAGGED, bool LAYER>
+__global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a) {
+    __shared__ RowSums sh[SEVERAL ? 32 : 1];
     int phase = 0;
-    const unsigned lanes = NW == 1 ? (unsigned)a.lanes : kThreads;
-    const unsigned lane = threadIdx.x & (lanes - 1);
-    const unsigned row = NW == 1 ? blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes : blockIdx.x;
+    clear_row_sums<SEVERAL>(sh);
+    const unsigned lanes = a.lanes;
+    const unsigned lane = SEVERAL ? threadIdx.x : threadIdx.x & (lanes - 1);
+    const unsigned row = SEVERAL ? blockIdx.x : blockIdx.x * (THREADS / lanes) + threadIdx.x / lanes;
     const bool live = row < a.rows;                      // (idle lanes still take part in the reductions)
     const unsigned n = live ? row : 0;
+    const bool inside = n + 1 < a.rows && a.width >= VEC;
     float v[C][VEC], x[C][VEC];
     int in[C];                                           // elements of each piece
 #pragma unroll
@@ -66,20 +73,20 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_norm_kernel(Nor
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[c][i] = x[c][i] = 0.0f;
         if (in[c]) {
-            load_piece<T, VEC, RAGGED>((const T*)a.x + (long long)n * a.x_stride + col, in[c], x[c]);
-            if (a.b) load_piece<T, VEC, RAGGED>((const T*)a.b + (long long)n * a.b_stride + col, in[c], v[c]);
+            load_piece<T, VEC, RAGGED>((const T*)a.x + (long long)n * a.x_stride + col, in[c], inside, x[c]);
+            if (a.b) load_piece<T, VEC, RAGGED>((const T*)a.b + (long long)n * a.b_stride + col, in[c], inside, v[c]);
         }
     }
     if (a.post) {
         float mean = 0.0f;
-        if (a.layer) {
+        if (LAYER) {
             float s[1] = {0.0f};
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) s[0] += v[c][i];
-            row_sums<1, NW>(s, lanes, sh, phase);
-            mean = s[0] * a.inv_width;
+            row_sums<1, SEVERAL>(s, lanes, sh, phase);
+            mean = s[0] / a.width_f;
         }
         float s[1] = {0.0f};
 #pragma unroll
@@ -89,7 +96,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_norm_kernel(Nor
                 v[c][i] = (RAGGED ? i < in[c] : in[c] > 0) ? v[c][i] - mean : 0.0f;
                 s[0] += v[c][i] * v[c][i];
             }
-        row_sums<1, NW>(s, lanes, sh, phase);
+        row_sums<1, SEVERAL>(s, lanes, sh, phase);
         const float r = 1.0f / sqrtf(s[0] * a.inv_width + a.eps);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -116,14 +123,14 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_norm_kernel(Nor
     }
     if (!a.y) return;
     float mean = 0.0f;
-    if (a.layer) {
+    if (LAYER) {
         float s[1] = {0.0f};
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) s[0] += v[c][i];
-        row_sums<1, NW>(s, lanes, sh, phase);
-        mean = s[0] * a.inv_width;
+        row_sums<1, SEVERAL>(s, lanes, sh, phase);
+        mean = s[0] / a.width_f;
     }
     float s[1] = {0.0f};
 #pragma unroll
@@ -133,7 +140,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_norm_kernel(Nor
             v[c][i] = (RAGGED ? i < in[c] : in[c] > 0) ? v[c][i] - mean : 0.0f;
             s[0] += v[c][i] * v[c][i];
         }
-    row_sums<1, NW>(s, lanes, sh, phase);
+    row_sums<1, SEVERAL>(s, lanes, sh, phase);
     const float r = 1.0f / sqrtf(s[0] * a.inv_width + a.eps);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -149,22 +156,25 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_norm_kernel(Nor
     }
 }
 
-// Backward.  A workgroup (with NW = 1: each group of lanes of it) takes the rows of a part one after the
-// other and keeps the part's sums over rows in registers; they go to a.parts at its end, and
-// block_norm_merge_kernel adds the parts in order.  BIAS: the sums of dz and dq are wanted.
-template <class T, int VEC, int C, int NW, bool RAGGED, bool BIAS>
-__global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_norm_grad_kernel(NormArgs a) {
-    constexpr int kThreads = NW == 1 ? 256 : NW * 64;
-    __shared__ float sh[NW == 1 ? 1 : 2 * kRowSumsMax * NW];
+// Backward.  A workgroup (not SEVERAL: each group of lanes of it) takes the rows of a part one after the
+// other, the next row in flight while one is worked on, and keeps the part's sums over rows in registers;
+// they go to a.parts at its end, and block_norm_merge_kernel adds the parts in order.  BIAS: the sums of
+// dz and dq are wanted.
+template <class T, int VEC, int C, int THREADS, bool SEVERAL, bool RAGGED, bool LAYER, bool BIAS>
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4))) void block_norm_grad_kernel(NormArgs a) {
+    typedef typename VecOf<T, VEC>::type Raw;
+    __shared__ RowSums sh[SEVERAL ? 32 : 1];
+    extern __shared__ float4 lds4[];
+    float* lds = reinterpret_cast<float*>(lds4);
     int phase = 0;
-    const unsigned lanes = NW == 1 ? (unsigned)a.lanes : kThreads;
-    const unsigned lane = threadIdx.x & (lanes - 1);
-    const unsigned part = NW == 1 ? blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes : blockIdx.x;
+    clear_row_sums<SEVERAL>(sh);
+    const unsigned lanes = a.lanes;
+    const unsigned lane = SEVERAL ? threadIdx.x : threadIdx.x & (lanes - 1);
+    const unsigned part = SEVERAL ? blockIdx.x : blockIdx.x * (THREADS / lanes) + threadIdx.x / lanes;
     const unsigned span = part / a.parts_per_span;
     const unsigned first = span * a.span_rows + (part - span * a.parts_per_span) * a.per_part;
     const unsigned span_end = min(a.rows, (span + 1) * a.span_rows);
     const unsigned last = first < span_end ? min(span_end, first + a.per_part) : first;
-    // (every group of lanes of a workgroup makes the same number of turns)
     float sw[C][VEC], sp[C][VEC], sg[C][VEC], sz[BIAS ? C : 1][VEC], sq[BIAS ? C : 1][VEC];
     int in[C];                                           // elements of each piece
 #pragma unroll
@@ -176,30 +186,67 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_norm_grad_kerne
             if constexpr (BIAS) sz[c][i] = sq[c][i] = 0.0f;
         }
     }
-    for (unsigned turn = 0; turn < a.per_part; ++turn) {
-        const bool live = first + turn < last;
-        if constexpr (NW > 1) {
-            if (!live) break;
-        }
-        const unsigned n = live ? first + turn : 0;
-        float h[C][VEC], b[C][VEC], d[C][VEC], t[C][VEC];
+    Raw rh[C], rt[C], rb[C], rd[C];
+    auto fetch = [&](unsigned n, bool live) {
+        const bool inside = n + 1 < a.rows && a.width >= VEC;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const unsigned col = (c * lanes + lane) * VEC;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) h[c][i] = b[c][i] = d[c][i] = t[c][i] = 0.0f;
-            if (live && in[c]) {
-                if (a.dy) {
-                    load_piece<T, VEC, RAGGED>((const T*)a.h + (long long)n * a.h_stride + col, in[c], h[c]);
-                    load_piece<T, VEC, RAGGED>((const T*)a.dy + (long long)n * a.dy_stride + col, in[c], t[c]);
-                }
-                if (a.b) load_piece<T, VEC, RAGGED>((const T*)a.b + (long long)n * a.b_stride + col, in[c], b[c]);
-                if (a.dh) load_piece<T, VEC, RAGGED>((const T*)a.dh + (long long)n * a.dh_stride + col, in[c], d[c]);
-            }
+            const int count = live ? in[c] : 0;
+            rh[c] = load_raw<T, VEC, RAGGED>((const T*)a.h + (long long)n * a.h_stride + col, a.dy ? count : 0, inside);
+            rt[c] = load_raw<T, VEC, RAGGED>((const T*)a.dy + (long long)n * a.dy_stride + col, a.dy ? count : 0, inside);
+            rb[c] = load_raw<T, VEC, RAGGED>((const T*)a.b + (long long)n * a.b_stride + col, a.b ? count : 0, inside);
+            rd[c] = load_raw<T, VEC, RAGGED>((const T*)a.dh + (long long)n * a.dh_stride + col, a.dh ? count : 0, inside);
         }
-        float bmean = 0.0f, brs = 1.0f;
-        // the norm after the block: its statistics, and d
-        if (a.layer) {
+    };
+    fetch(first, first < last);
+    float* lds_post_gain = lds + (a.in_lds & kVecGain ? a.lds_stride : 0);
+    float* lds_post_bias = lds_post_gain + (a.in_lds & kVecPostGain ? a.lds_stride : 0);
+    float* lds_gate = lds_post_bias + (a.in_lds & kVecPostBias ? a.lds_stride : 0);
+    // Gains, bias and gate are needed right behind the reductions, several times a row: a lane keeps its pieces of
+    // them in LDS (where registers are short; every lane reads back what it wrote, so there is no barrier).  A
+    // row of 4096 bf16 elements, 16384 of them: 299 us with loads from the second-level cache each time, 202 so.
+    if (a.in_lds) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if (!in[c]) continue;
+            const unsigned col = (c * lanes + lane) * VEC;
+            float w[VEC], p[VEC], q[VEC], g[VEC];
+            if (a.in_lds & kVecGain) load_param<T, VEC, RAGGED>(a.gain, col, in[c], a.param_f32, 1.0f, w);
+            if (a.in_lds & kVecPostGain) load_param<T, VEC, RAGGED>(a.post_gain, col, in[c], a.param_f32, 1.0f, p);
+            if (a.in_lds & kVecPostBias) load_param<T, VEC, RAGGED>(a.post_bias, col, in[c], a.param_f32, 0.0f, q);
+            if (a.in_lds & kVecGate)                     // (a part's rows share a gate row where the gate is copied)
+                load_param<T, VEC, RAGGED>(a.gate, (long long)(min(first, a.rows - 1) / a.gate_rows) * a.gate_stride + col, in[c], a.param_f32, 1.0f, g);
+            if (a.in_lds & kVecGain) store_from_float<float, VEC>(lds + col, w);
+            if (a.in_lds & kVecPostGain) store_from_float<float, VEC>(lds_post_gain + col, p);
+            if (a.in_lds & kVecPostBias) store_from_float<float, VEC>(lds_post_bias + col, q);
+            if (a.in_lds & kVecGate) store_from_float<float, VEC>(lds_gate + col, g);
+        }
+    }
+    auto param = [&](int bit, const float* copy, const void* p, long long at, unsigned col, int count, float other, float (&out)[VEC]) {
+        if (a.in_lds & bit) load_as_float<float, VEC>(copy + col, out);
+        else load_param<T, VEC, RAGGED>(p, at, count, a.param_f32, other, out);
+    };
+    // (every group of lanes of a workgroup makes the same number of turns)
+    for (unsigned turn = 0; turn < a.per_part; ++turn) {
+        const bool live = first + turn < last;
+        if constexpr (SEVERAL) {
+            if (!live) break;
+        }
+        const unsigned n = first + turn;
+        float h[C][VEC], t[C][VEC], b[C][VEC], d[C][VEC];
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                h[c][i] = (float)rh[c][i];
+                t[c][i] = (float)rt[c][i];
+                b[c][i] = (float)rb[c][i];
+                d[c][i] = (float)rd[c][i];
+            }
+        fetch(n + 1, n + 1 < last);
+        float brs = 1.0f;
+        if (LAYER) {
             float s[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < C; ++c)
@@ -208,9 +255,8 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_norm_grad_kerne
                     s[0] += h[c][i];
                     s[1] += b[c][i];
                 }
-            row_sums<2, NW>(s, lanes, sh, phase);
-            const float hmean = s[0] * a.inv_width;
-            bmean = a.post ? s[1] * a.inv_width : 0.0f;
+            row_sums<2, SEVERAL>(s, lanes, sh, phase);
+            const float hmean = s[0] / a.width_f, bmean = a.post ? s[1] / a.width_f : 0.0f;
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -220,14 +266,14 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_norm_grad_kerne
                 }
         }
         {
-            // sums of h^2, t h and t (t = dy w), b^2
-            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            // sums of h^2, t h (t = dy w), b^2 and, for the layer norm, t
+            float s[LAYER ? 4 : 3] = {};
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 float w[VEC];
                 const unsigned col = (c * lanes + lane) * VEC;
-                if (live && in[c]) {
-                    load_param<T, VEC, RAGGED>(a.gain, col, in[c], a.param_f32, 1.0f, w);
+                if (in[c]) {
+                    param(kVecGain, lds, a.gain, col, col, in[c], 1.0f, w);
                 } else {
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) w[i] = 0.0f;
@@ -237,28 +283,28 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_norm_grad_kerne
                     const float tw = t[c][i] * w[i];
                     s[0] += h[c][i] * h[c][i];
                     s[1] += tw * h[c][i];
-                    s[2] += tw;
-                    s[3] += b[c][i] * b[c][i];
+                    s[2] += b[c][i] * b[c][i];
+                    if constexpr (LAYER) s[3] += tw;
                 }
             }
-            row_sums<4, NW>(s, lanes, sh, phase);
+            row_sums<LAYER ? 4 : 3, SEVERAL>(s, lanes, sh, phase);
             const float r = 1.0f / sqrtf(s[0] * a.inv_width + a.eps);
-            if (a.post) brs = 1.0f / sqrtf(s[3] * a.inv_width + a.eps);
-            if (a.dy) {
+            if (a.post) brs = 1.0f / sqrtf(s[2] * a.inv_width + a.eps);
+            if (a.dy && live) {
                 const float along = s[1] * r * a.inv_width;              // mean(t hh)
-                const float level = a.layer ? s[2] * a.inv_width : 0.0f;
+                const float level = LAYER ? s[LAYER ? 3 : 0] * a.inv_width : 0.0f;
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
                     float w[VEC];
                     const unsigned col = (c * lanes + lane) * VEC;
-                    if (live && in[c]) {
-                        load_param<T, VEC, RAGGED>(a.gain, col, in[c], a.param_f32, 1.0f, w);
+                    if (in[c]) {
+                        param(kVecGain, lds, a.gain, col, col, in[c], 1.0f, w);
 #pragma unroll
                         for (int i = 0; i < VEC; ++i) {
                             const float hh = h[c][i] * r;
                             sw[c][i] += t[c][i] * hh;
                             if constexpr (BIAS) sz[c][i] += t[c][i];
-                            if (!RAGGED || i < in[c]) d[c][i] += r * (t[c][i] * w[i] - hh * along - level);
+                            if (!RAGGED || i < in[c]) d[c][i] += r * (t[c][i] * w[i] - hh * along - (LAYER ? level : 0.0f));
                         }
                     }
                 }
@@ -275,16 +321,16 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_norm_grad_kerne
             }
         }
         if (!a.db) continue;
-        const unsigned gate_row = a.gate ? n / a.gate_rows : 0;
-        float s[2] = {0.0f, 0.0f};
+        const unsigned gate_row = a.gate && live ? n / a.gate_rows : 0;
+        float s[LAYER ? 2 : 1] = {};
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const unsigned col = (c * lanes + lane) * VEC;
             if (live && in[c]) {
                 float g[VEC], p[VEC], q[VEC];
-                load_param<T, VEC, RAGGED>(a.gate, a.gate ? (long long)gate_row * a.gate_stride + col : 0, in[c], a.param_f32, 1.0f, g);
-                load_param<T, VEC, RAGGED>(a.post_gain, col, in[c], a.param_f32, 1.0f, p);
-                load_param<T, VEC, RAGGED>(a.post_bias, col, in[c], a.param_f32, 0.0f, q);
+                param(kVecGate, lds_gate, a.gate, a.gate ? (long long)gate_row * a.gate_stride + col : 0, col, in[c], 1.0f, g);
+                param(kVecPostGain, lds_post_gain, a.post_gain, col, col, in[c], 1.0f, p);
+                param(kVecPostBias, lds_post_bias, a.post_bias, col, col, in[c], 0.0f, q);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
                     const float bh = b[c][i] * brs;
@@ -295,17 +341,17 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_norm_grad_kerne
                     if constexpr (BIAS) sq[c][i] += e;
                     d[c][i] = e * p[i];
                     s[0] += d[c][i] * bh;
-                    s[1] += d[c][i];
+                    if constexpr (LAYER) s[LAYER ? 1 : 0] += d[c][i];
                 }
             }
         }
         if (a.post) {
-            row_sums<2, NW>(s, lanes, sh, phase);
-            const float along = s[0] * a.inv_width, level = a.layer ? s[1] * a.inv_width : 0.0f;
+            row_sums<LAYER ? 2 : 1, SEVERAL>(s, lanes, sh, phase);
+            const float along = s[0] * a.inv_width, level = LAYER ? s[LAYER ? 1 : 0] * a.inv_width : 0.0f;
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) d[c][i] = brs * (d[c][i] - b[c][i] * along - level);
+                for (int i = 0; i < VEC; ++i) d[c][i] = brs * (d[c][i] - b[c][i] * along - (LAYER ? level : 0.0f));
         }
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -391,44 +437,55 @@ __global__ __launch_bounds__(1024) void block_norm_merge_kernel(NormMergeArgs a)
     else ((T*)a.out[vec])[col] = (T)acc;
 }
 
-// The shape of the kernel that a row takes: C pieces of VEC elements a lane, `waves` wavefronts (one: `lanes`
-// lanes of it).  ragged: rows that do not start, or end, on 16-byte boundaries.
+// The shape of the kernel that a row takes: C pieces of VEC elements a lane on `lanes` lanes (whole wavefronts,
+// or a power of two up to 64).  ragged: rows that do not start, or end, on 16-byte boundaries.
 struct NormShape {
-    int pieces, waves, lanes;
+    int pieces, lanes;
     bool ragged;
+    bool several() const { return lanes > 64; }
+    unsigned threads() const { return several() ? (unsigned)lanes : 256u; }
+    unsigned rows_a_workgroup() const { return several() ? 1u : 256u / (unsigned)lanes; }
 };
 
-// One translation unit for each storage type; `backward` chooses the kernel.
-NGH_INTERNAL int launch_norm_f32(const NormShape& s, const NormArgs& a, bool backward, bool bias, unsigned grid, hipStream_t stream);
-NGH_INTERNAL int launch_norm_f16(const NormShape& s, const NormArgs& a, bool backward, bool bias, unsigned grid, hipStream_t stream);
-NGH_INTERNAL int launch_norm_bf16(const NormShape& s, const NormArgs& a, bool backward, bool bias, unsigned grid, hipStream_t stream);
+// One translation unit for each storage type.
+enum NormPass { kNormForward, kNormBackward, kNormBackwardBias };
+NGH_INTERNAL int launch_norm_f32(const NormShape& s, const NormArgs& a, NormPass pass, bool layer, unsigned grid, hipStream_t stream);
+NGH_INTERNAL int launch_norm_f16(const NormShape& s, const NormArgs& a, NormPass pass, bool layer, unsigned grid, hipStream_t stream);
+NGH_INTERNAL int launch_norm_bf16(const NormShape& s, const NormArgs& a, NormPass pass, bool layer, unsigned grid, hipStream_t stream);
 
-template <class T, int VEC, int C, int NW, bool RAGGED>
-void launch_norm_kernel(const NormArgs& a, bool backward, bool bias, unsigned grid, hipStream_t stream) {
-    const dim3 block(NW == 1 ? 256 : NW * 64);
-    if (!backward) hipLaunchKernelGGL((block_norm_kernel<T, VEC, C, NW, RAGGED>), dim3(grid), block, 0, stream, a);
-    else if (bias) hipLaunchKernelGGL((block_norm_grad_kernel<T, VEC, C, NW, RAGGED, true>), dim3(grid), block, 0, stream, a);
-    else hipLaunchKernelGGL((block_norm_grad_kernel<T, VEC, C, NW, RAGGED, false>), dim3(grid), block, 0, stream, a);
+template <class T, int VEC, int C, int THREADS, bool SEVERAL, bool RAGGED, bool LAYER>
+void launch_norm_kernel(const NormShape& s, const NormArgs& a, NormPass pass, unsigned grid, hipStream_t stream) {
+    const dim3 block(s.threads());
+    const unsigned lds = (unsigned)__builtin_popcount((unsigned)a.in_lds) * a.lds_stride * 4;
+    if (pass == kNormForward) hipLaunchKernelGGL((block_norm_kernel<T, VEC, C, THREADS, SEVERAL, RAGGED, LAYER>), dim3(grid), block, 0, stream, a);
+    else if (pass == kNormBackward)
+        hipLaunchKernelGGL((block_norm_grad_kernel<T, VEC, C, THREADS, SEVERAL, RAGGED, LAYER, false>), dim3(grid), block, lds, stream, a);
+    else hipLaunchKernelGGL((block_norm_grad_kernel<T, VEC, C, THREADS, SEVERAL, RAGGED, LAYER, true>), dim3(grid), block, lds, stream, a);
 }
 
-// 8 elements a lane on up to 8 wavefronts (rows of up to 4096 elements), 16 on 8 or 16.
-template <class T, bool RAGGED>
-int launch_norm(const NormShape& s, const NormArgs& a, bool backward, bool bias, unsigned grid, hipStream_t stream) {
-    constexpr int kVec = 16 / sizeof(T), kEight = 8 / kVec;
-    if (s.pieces == kEight) {
-        switch (s.waves) {
-            case 1: launch_norm_kernel<T, kVec, kEight, 1, RAGGED>(a, backward, bias, grid, stream); break;
-            case 2: launch_norm_kernel<T, kVec, kEight, 2, RAGGED>(a, backward, bias, grid, stream); break;
-            case 4: launch_norm_kernel<T, kVec, kEight, 4, RAGGED>(a, backward, bias, grid, stream); break;
-            default: launch_norm_kernel<T, kVec, kEight, 8, RAGGED>(a, backward, bias, grid, stream); break;
-        }
-    } else if (s.waves == 8) {
-        launch_norm_kernel<T, kVec, 2 * kEight, 8, RAGGED>(a, backward, bias, grid, stream);
+// The pieces a lane may hold: one (rows of up to 16 KiB: at most 1024 lanes), two, and four of 4 elements.
+template <class T, bool RAGGED, bool LAYER>
+int launch_norm_shape(const NormShape& s, const NormArgs& a, NormPass pass, unsigned grid, hipStream_t stream) {
+    constexpr int kVec = 16 / sizeof(T);
+    if (s.pieces == 1) {
+        if (!s.several()) launch_norm_kernel<T, kVec, 1, 256, false, RAGGED, LAYER>(s, a, pass, grid, stream);
+        else if (s.lanes <= 256) launch_norm_kernel<T, kVec, 1, 256, true, RAGGED, LAYER>(s, a, pass, grid, stream);
+        else if (s.lanes <= 512) launch_norm_kernel<T, kVec, 1, 512, true, RAGGED, LAYER>(s, a, pass, grid, stream);
+        else launch_norm_kernel<T, kVec, 1, 1024, true, RAGGED, LAYER>(s, a, pass, grid, stream);
+    } else if (s.pieces == 2) {
+        launch_norm_kernel<T, kVec, 2, 1024, true, RAGGED, LAYER>(s, a, pass, grid, stream);
     } else {
-        launch_norm_kernel<T, kVec, 2 * kEight, 16, RAGGED>(a, backward, bias, grid, stream);
+        if constexpr (kVec == 4) launch_norm_kernel<T, kVec, 4, 1024, true, RAGGED, LAYER>(s, a, pass, grid, stream);
     }
     NGH_HIP_TRY(hipGetLastError());
     return NGH_OK;
+}
+
+template <class T>
+int launch_norm(const NormShape& s, const NormArgs& a, NormPass pass, bool layer, unsigned grid, hipStream_t stream) {
+    if (s.ragged)
+        return layer ? launch_norm_shape<T, true, true>(s, a, pass, grid, stream) : launch_norm_shape<T, true, false>(s, a, pass, grid, stream);
+    return layer ? launch_norm_shape<T, false, true>(s, a, pass, grid, stream) : launch_norm_shape<T, false, false>(s, a, pass, grid, stream);
 }
 
 }  // namespace ngh

@@ -125,12 +125,12 @@ NormShape shape_of(const ngh_block_norm_spec* s, bool grad) {
         whole = whole && (uintptr_t)v[i].p % piece == 0 && (v[i].rows <= 1 || v[i].stride * v[i].item % piece == 0);
     }
     f.ragged = !whole;
-    const int per_lane = s->width > 8 * 64 * 8 ? 16 : 8;
-    f.pieces = per_lane / vec;
+    f.pieces = 1;
+    while (1024 * vec * f.pieces < s->width) f.pieces *= 2;
+    const int per_lane = vec * f.pieces;
     f.lanes = 1;
     while (f.lanes < 64 && f.lanes * per_lane < s->width) f.lanes *= 2;
-    f.waves = 1;
-    while (f.waves * 64 * per_lane < s->width) f.waves *= 2;
+    if (f.lanes * per_lane < s->width) f.lanes = (int)((s->width + per_lane * 64 - 1) / (per_lane * 64)) * 64;
     return f;
 }
 
@@ -144,18 +144,19 @@ void fill_args(const ngh_block_norm_spec* s, const NormShape& f, NormArgs& a) {
     a.width = (unsigned)s->width;
     a.gate_rows = (unsigned)std::max<int64_t>(1, s->gate_rows);
     a.lanes = f.lanes;
-    a.layer = s->kind == NGH_NORM_LAYER;
     a.post = s->post_norm != 0;
     a.param_f32 = s->param_dtype == NGH_F32;
     a.eps = s->eps;
     a.alpha = s->residual_scale;
-    a.inv_width = 1.0f / (float)s->width;
+    a.width_f = (float)s->width;
+    a.inv_width = 1.0f / a.width_f;
 }
 
-int launch(const ngh_block_norm_spec* s, const NormShape& f, const NormArgs& a, bool backward, bool bias, unsigned grid, hipStream_t stream) {
-    if (s->dtype == NGH_F32) return launch_norm_f32(f, a, backward, bias, grid, stream);
-    if (s->dtype == NGH_F16) return launch_norm_f16(f, a, backward, bias, grid, stream);
-    return launch_norm_bf16(f, a, backward, bias, grid, stream);
+int launch(const ngh_block_norm_spec* s, const NormShape& f, const NormArgs& a, NormPass pass, unsigned grid, hipStream_t stream) {
+    const bool layer = s->kind == NGH_NORM_LAYER;
+    if (s->dtype == NGH_F32) return launch_norm_f32(f, a, pass, layer, grid, stream);
+    if (s->dtype == NGH_F16) return launch_norm_f16(f, a, pass, layer, grid, stream);
+    return launch_norm_bf16(f, a, pass, layer, grid, stream);
 }
 
 // How the rows of the backward pass are dealt, and where the sums of the parts lie.
@@ -173,11 +174,12 @@ GradPlan plan_grad(const ngh_block_norm_spec* s, int cus) {
     g.vectors = (s->dgain ? kVecGain : 0) | (s->dbias ? kVecBias : 0) | (s->dpost_gain ? kVecPostGain : 0) | (s->dpost_bias ? kVecPostBias : 0);
     g.bias = s->dbias || s->dpost_bias;
     const unsigned rows = (unsigned)s->rows;
-    // Two workgroups a compute unit, but at least 8 rows a part: a part's sums are written in fp32 and
-    // read once more.
-    const unsigned groups = g.shape.waves == 1 ? 256u / g.shape.lanes : 1u;              // parts a workgroup holds
-    const unsigned want = 2u * cus * groups;
-    g.per_part = std::max(8u, (rows + want - 1) / std::max(1u, want));
+    // 16 wavefronts a compute unit (what the registers allow), but at least 8 rows a part, for a part's sums are
+    // written in fp32 and read once more; fewer, down to 2, where else compute units would have no part.
+    const unsigned groups = g.shape.rows_a_workgroup();                                  // parts a workgroup holds
+    const unsigned want = std::max(1u, 1024u / g.shape.threads()) * cus * groups;
+    const unsigned least = std::min(8u, std::max(2u, rows / (2u * cus * groups)));
+    g.per_part = std::max(least, (rows + want - 1) / want);
     const unsigned gate_rows = (unsigned)std::max<int64_t>(1, s->gate_rows);
     g.gate_whole = !s->dgate || gate_rows < 2 * g.per_part;
     g.span_rows = g.gate_whole ? std::max(1u, rows) : gate_rows;
@@ -229,8 +231,8 @@ int ngh_block_norm(ngh_context* ctx, const ngh_block_norm_spec* spec) {
     const NormShape f = shape_of(spec, false);
     NormArgs a;
     fill_args(spec, f, a);
-    const unsigned per_wg = f.waves == 1 ? 256u / f.lanes : 1u;
-    return launch(spec, f, a, false, false, (a.rows + per_wg - 1) / per_wg, c.stream);
+    const unsigned per_wg = f.rows_a_workgroup();
+    return launch(spec, f, a, kNormForward, (a.rows + per_wg - 1) / per_wg, c.stream);
 }
 
 int ngh_block_norm_grad_workspace(const ngh_block_norm_spec* spec, size_t* out_bytes) {
@@ -264,8 +266,21 @@ int ngh_block_norm_grad(ngh_context* ctx, const ngh_block_norm_spec* spec) {
     a.per_part = g.per_part;
     a.vectors = g.vectors;
     a.gate_whole = g.gate_whole;
+    // Vectors copied to LDS, as far as 48 KiB go (64 KiB a workgroup without further ado, the reductions' words
+    // among it); the gate where a part's rows share one row of it.
+    a.lds_stride = (a.width + 7) / 8 * 8;
+    const int wanted[4][2] = {{kVecGain, spec->gain != nullptr},
+                              {kVecPostGain, spec->post_gain != nullptr},
+                              {kVecGate, spec->gate != nullptr && (spec->gate_rows == spec->rows || (!g.gate_whole && g.shape.rows_a_workgroup() == 1))},
+                              {kVecPostBias, spec->post_bias != nullptr}};
+    size_t room = 48u << 10;
+    for (const auto& w : wanted)
+        if (w[1] && a.lds_stride * 4 <= room) {
+            a.in_lds |= w[0];
+            room -= a.lds_stride * 4;
+        }
     if (spec->rows) {
-        const int lrc = launch(spec, g.shape, a, true, g.bias, g.grid, c.stream);
+        const int lrc = launch(spec, g.shape, a, g.bias ? kNormBackwardBias : kNormBackward, g.grid, c.stream);
         if (lrc != NGH_OK) return lrc;
     }
     if (!g.vectors) return NGH_OK;

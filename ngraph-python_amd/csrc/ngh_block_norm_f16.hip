@@ -2,7 +2,7 @@
 #include "ngh_block_norm.h"
 
 namespace ngh {
-int launch_norm_f16(const NormShape& s, const NormArgs& a, bool backward, bool bias, unsigned grid, hipStream_t stream) {
-    return s.ragged ? launch_norm<f16_t, true>(s, a, backward, bias, grid, stream) : launch_norm<f16_t, false>(s, a, backward, bias, grid, stream);
+int launch_norm_f16(const NormShape& s, const NormArgs& a, NormPass pass, bool layer, unsigned grid, hipStream_t stream) {
+    return launch_norm<f16_t>(s, a, pass, layer, grid, stream);
 }
 }  // namespace ngh

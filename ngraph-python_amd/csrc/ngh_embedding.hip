@@ -64,13 +64,14 @@ __global__ __launch_bounds__(kEmbBlock) void embedding_kernel(LookupArgs a) {
     const unsigned per_wg = kEmbBlock / a.lanes;
     const unsigned first = (blockIdx.x * per_wg + group) * kLookupRows;
     const TIn* src[kLookupRows];
-    bool live[kLookupRows], has[kLookupRows];
+    bool live[kLookupRows], has[kLookupRows], inside[kLookupRows];
 #pragma unroll
     for (int r = 0; r < kLookupRows; ++r) {
         const unsigned n = first + r;
         live[r] = n < a.rows;
         const int t = live[r] ? a.tokens[n] : -1;
         has[r] = live[r] && (unsigned)t < a.vocab && t != a.pad;
+        inside[r] = has[r] && (unsigned)t + 1 < a.vocab && a.width >= VEC;
         src[r] = (const TIn*)a.table + (has[r] ? (long long)t * a.table_stride : 0);
     }
     for (unsigned c = lane; c < a.chunks; c += a.lanes) {
@@ -79,7 +80,7 @@ __global__ __launch_bounds__(kEmbBlock) void embedding_kernel(LookupArgs a) {
 #pragma unroll
         for (int r = 0; r < kLookupRows; ++r) {
             if (has[r]) {
-                load_piece<TIn, VEC, RAGGED>(src[r] + (size_t)c * VEC, in, v[r]);
+                load_piece<TIn, VEC, RAGGED>(src[r] + (size_t)c * VEC, in, inside[r], v[r]);
             } else {
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) v[r][i] = 0.0f;
@@ -348,7 +349,7 @@ __device__ __forceinline__ void finish_row(const SumArgs& a, unsigned token, uns
     TOut* to = (TOut*)a.table + (long long)token * a.table_stride + col;
     float v[VEC];
     if (a.accumulate) {
-        load_piece<TOut, VEC, RAGGED>(to, in, v);
+        load_piece<TOut, VEC, RAGGED>(to, in, false, v);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[i] += a.scale * acc[i];
     } else {
@@ -356,23 +357,6 @@ __device__ __forceinline__ void finish_row(const SumArgs& a, unsigned token, uns
         for (int i = 0; i < VEC; ++i) v[i] = a.scale * acc[i];
     }
     store_piece<TOut, VEC, RAGGED>(to, in, v);
-}
-
-// A row's piece as it lies in memory, so that rows in flight take as few registers as bytes.
-template <class T, int VEC, bool RAGGED>
-__device__ __forceinline__ typename VecOf<T, VEC>::type load_raw(const T* p, int count) {
-    typename VecOf<T, VEC>::type v;
-    if (RAGGED ? count == VEC : count > 0) {
-        if constexpr (RAGGED) v = *reinterpret_cast<const typename VecOf<T, VEC>::loose*>(p);
-        else v = *reinterpret_cast<const typename VecOf<T, VEC>::type*>(p);
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            v[i] = (T)0.0f;
-            if (RAGGED && i < count) v[i] = p[i];
-        }
-    }
-    return v;
 }
 
 constexpr int kUnitMax = 64;       // places of a unit: a lane holds one
@@ -451,10 +435,10 @@ __global__ __launch_bounds__(kEmbBlock) void embedding_sum_kernel(SumArgs a, uns
         for (int k = 0; k < kAhead; ++k) {
             if (i + k < valid) {
                 const unsigned place = __builtin_amdgcn_readlane(my_place, i + k);
-                to[k] = load_raw<TIn, VEC, RAGGED>(dy + (long long)place * a.dy_stride, in);
+                to[k] = load_raw<TIn, VEC, RAGGED>(dy + (long long)place * a.dy_stride, in, place + 1 < a.n && a.width >= VEC);
                 if constexpr (ADD) {
                     const unsigned key = key_at(i + k);
-                    if (key != key_at(i + k + 1)) old[k] = load_raw<TOut, VEC, RAGGED>(table + (long long)key * a.table_stride, in);
+                    if (key != key_at(i + k + 1)) old[k] = load_raw<TOut, VEC, RAGGED>(table + (long long)key * a.table_stride, in, false);
                 }
             }
         }
@@ -569,7 +553,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void embedding_few_kernel(SumArgs a
             for (int k = 0; k < kAhead; ++k) {
                 if (e + k < e1) {
                     const unsigned place = __builtin_amdgcn_readfirstlane((unsigned)found[w][e + k]);
-                    rows[k] = load_raw<TIn, VEC, RAGGED>(dy + (long long)place * a.dy_stride, in);
+                    rows[k] = load_raw<TIn, VEC, RAGGED>(dy + (long long)place * a.dy_stride, in, place + 1 < a.n && a.width >= VEC);
                 }
             }
 #pragma unroll

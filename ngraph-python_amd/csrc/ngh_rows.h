@@ -45,18 +45,34 @@ __device__ __forceinline__ void store_from_float(T* p, const float (&in)[V]) {
 }
 
 // The first `count` (0 .. V) of V elements, zeros behind them.  RAGGED: rows start on any boundary
-// and may end inside a piece; else count is 0 or V.
+// and may end inside a piece; else count is 0 or V.  A piece that ends behind its row is still loaded
+// whole where that stays inside the operand (`inside`: another row follows that is no shorter than a
+// piece), and only element by element where it does not: in the last row.
 template <class T, int V, bool RAGGED>
-__device__ __forceinline__ void load_piece(const T* p, int count, float (&out)[V]) {
-    if (RAGGED ? count == V : count > 0) {
-        load_as_float<T, V, RAGGED>(p, out);
+__device__ __forceinline__ typename VecOf<T, V>::type load_raw(const T* p, int count, bool inside) {
+    typename VecOf<T, V>::type v;
+    if (!RAGGED ? count > 0 : count == V || (inside && count > 0)) {
+        if constexpr (RAGGED) v = *reinterpret_cast<const typename VecOf<T, V>::loose*>(p);
+        else v = *reinterpret_cast<const typename VecOf<T, V>::type*>(p);
+        if constexpr (RAGGED) {
+#pragma unroll
+            for (int i = 1; i < V; ++i) v[i] = i < count ? v[i] : (T)0.0f;
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            out[i] = 0.0f;
-            if (RAGGED && i < count) out[i] = (float)p[i];
+            v[i] = (T)0.0f;
+            if (RAGGED && i < count) v[i] = p[i];
         }
     }
+    return v;
+}
+
+template <class T, int V, bool RAGGED>
+__device__ __forceinline__ void load_piece(const T* p, int count, bool inside, float (&out)[V]) {
+    const typename VecOf<T, V>::type v = load_raw<T, V, RAGGED>(p, count, inside);
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = (float)v[i];
 }
 
 template <class T, int V, bool RAGGED>
@@ -77,37 +93,73 @@ __device__ __forceinline__ int piece_count(unsigned col, unsigned width) {
     else return col < width ? V : 0;
 }
 
-// The sum over the lanes of a row.  NW > 1: the row has NW whole wavefronts, which are the workgroup;
-// `sh` holds 2 x kRowSumsMax x NW floats and `phase` alternates, so one barrier a reduction is enough (a
-// wavefront that is a reduction ahead writes the other half).  NW == 1: `lanes` (a power of two up to
-// 64) consecutive lanes of a wavefront, no barrier.
-template <int N, int NW>
-__device__ __forceinline__ void row_sums(float (&v)[N], int lanes, float* sh, int& phase) {
-    if constexpr (NW == 1) {
-        for (int m = lanes >> 1; m > 0; m >>= 1) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], m, 64);
-        }
+// x plus the x of the lane's partner at distance 1, 2, 4, 8, 16 or 32, where the lanes at smaller
+// distances hold the same sum already: one instruction each within 16 lanes (the partner of a mirror is
+// not the lane at that distance but one with the same sum), two beyond.
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float x) {
+    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+
+template <int DISTANCE>
+__device__ __forceinline__ float add_partner(float x) {
+    if constexpr (DISTANCE == 1) return add_dpp<0xB1>(x);          // quad_perm 1,0,3,2
+    else if constexpr (DISTANCE == 2) return add_dpp<0x4E>(x);     // quad_perm 2,3,0,1
+    else if constexpr (DISTANCE == 4) return add_dpp<0x141>(x);    // row_half_mirror
+    else if constexpr (DISTANCE == 8) return add_dpp<0x140>(x);    // row_mirror
+    else if constexpr (DISTANCE == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
     } else {
-#pragma unroll
-        for (int m = 32; m > 0; m >>= 1) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], m, 64);
-        }
-        float* half = sh + phase * (kRowSumsMax * NW);
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+}
+
+// The sums over the lanes of a row of up to kRowSumsMax values.  SEVERAL: the row has several wavefronts
+// (up to 16), which are the workgroup; `sh` holds 2 x 16 entries that were cleared before the first
+// reduction (clear_row_sums) and `phase` alternates, so one barrier a reduction is enough (a wavefront that
+// is a reduction ahead writes the other half).  Else `lanes` (a power of two up to 64) consecutive lanes
+// of a wavefront, no barrier.  A value costs 8 vector instructions within a wavefront and 5 across them;
+// with a permutation through LDS for every step they were a fifth of the backward kernel.
+struct alignas(16) RowSums {
+    float v[kRowSumsMax];
+};
+
+template <bool SEVERAL>
+__device__ __forceinline__ void clear_row_sums(RowSums* sh) {
+    if constexpr (SEVERAL) {
+        if (threadIdx.x < 2 * 16 * kRowSumsMax) reinterpret_cast<float*>(sh)[threadIdx.x] = 0.0f;
+        if (blockDim.x < 2 * 16 * kRowSumsMax && threadIdx.x + blockDim.x < 2 * 16 * kRowSumsMax)
+            reinterpret_cast<float*>(sh)[threadIdx.x + blockDim.x] = 0.0f;
+        __syncthreads();
+    }
+}
+
+template <int N, bool SEVERAL>
+__device__ __forceinline__ void row_sums(float (&v)[N], int lanes, RowSums* sh, int& phase) {
+#define NGH_ROW_SUMS_STEP(DISTANCE)          \
+    if (SEVERAL || lanes > DISTANCE) {       \
+        _Pragma("unroll") for (int i = 0; i < N; ++i) v[i] = add_partner<DISTANCE>(v[i]); \
+    }
+    NGH_ROW_SUMS_STEP(1)
+    NGH_ROW_SUMS_STEP(2)
+    NGH_ROW_SUMS_STEP(4)
+    NGH_ROW_SUMS_STEP(8)
+    NGH_ROW_SUMS_STEP(16)
+    NGH_ROW_SUMS_STEP(32)
+#undef NGH_ROW_SUMS_STEP
+    if constexpr (SEVERAL) {
+        RowSums* half = sh + phase * 16;
         phase ^= 1;
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) half[i * NW + (threadIdx.x >> 6)] = v[i];
+            for (int i = 0; i < N; ++i) half[threadIdx.x >> 6].v[i] = v[i];
         }
         __syncthreads();
+        const RowSums all = half[threadIdx.x & 15];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float s = half[i * NW];
-#pragma unroll
-            for (int w = 1; w < NW; ++w) s += half[i * NW + w];
-            v[i] = s;
-        }
+        for (int i = 0; i < N; ++i) v[i] = add_partner<8>(add_partner<4>(add_partner<2>(add_partner<1>(all.v[i]))));
     }
 }
 
