@@ -30,10 +30,11 @@ struct NormArgs {
     int lanes;                     // along a row: whole wavefronts, or a power of two up to 64
     int post, param_f32;
     float eps, alpha, inv_width, width_f;      // (a mean is a quotient: a row of equal elements is all zeros behind it)
-    // backward: rows [part * per_part, ...) of a span of consecutive rows of one gate row, or several whole ones
-    unsigned span_rows, parts_per_span, per_part;
+    // backward: a part (a workgroup) has rows [part * per_part, ...) of a span of consecutive rows, those of one
+    // gate row or all; a group of lanes that makes up a row has per_group of them
+    unsigned span_rows, parts_per_span, per_part, per_group;
     int vectors;                   // sums a part writes: gain, bias, post gain, post bias, gate (bits), in this order
-    int gate_whole;                // a part holds whole gate rows and writes their gradients itself
+    int gate_whole;                // a group has whole gate rows and writes their gradients itself
     int in_lds;                    // vectors that the workgroup keeps in LDS (bits, kVec*)
     unsigned lds_stride;           // floats from one of them to the next
 };
@@ -158,8 +159,8 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a) {
 
 // Backward.  A workgroup (not SEVERAL: each group of lanes of it) takes the rows of a part one after the
 // other, the next row in flight while one is worked on, and keeps the part's sums over rows in registers;
-// they go to a.parts at its end, and block_norm_merge_kernel adds the parts in order.  BIAS: the sums of
-// dz and dq are wanted.
+// they go to a.parts at its end (of the groups of a workgroup joined in LDS, in order), and
+// block_norm_merge_kernel adds the parts in order.  BIAS: the sums of dz and dq are wanted.
 template <class T, int VEC, int C, int THREADS, bool SEVERAL, bool RAGGED, bool LAYER, bool BIAS>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4))) void block_norm_grad_kernel(NormArgs a) {
     typedef typename VecOf<T, VEC>::type Raw;
@@ -170,11 +171,12 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4))) vo
     clear_row_sums<SEVERAL>(sh);
     const unsigned lanes = a.lanes;
     const unsigned lane = SEVERAL ? threadIdx.x : threadIdx.x & (lanes - 1);
-    const unsigned part = SEVERAL ? blockIdx.x : blockIdx.x * (THREADS / lanes) + threadIdx.x / lanes;
+    const unsigned part = blockIdx.x, group = SEVERAL ? 0 : threadIdx.x / lanes;
     const unsigned span = part / a.parts_per_span;
-    const unsigned first = span * a.span_rows + (part - span * a.parts_per_span) * a.per_part;
-    const unsigned span_end = min(a.rows, (span + 1) * a.span_rows);
-    const unsigned last = first < span_end ? min(span_end, first + a.per_part) : first;
+    const unsigned part_first = span * a.span_rows + (part - span * a.parts_per_span) * a.per_part;
+    const unsigned part_end = min(min(a.rows, (span + 1) * a.span_rows), part_first + a.per_part);
+    const unsigned first = part_first + group * a.per_group;
+    const unsigned last = max(first, min(part_end, first + a.per_group));
     float sw[C][VEC], sp[C][VEC], sg[C][VEC], sz[BIAS ? C : 1][VEC], sq[BIAS ? C : 1][VEC];
     int in[C];                                           // elements of each piece
 #pragma unroll
@@ -216,7 +218,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4))) vo
             if (a.in_lds & kVecPostGain) load_param<T, VEC, RAGGED>(a.post_gain, col, in[c], a.param_f32, 1.0f, p);
             if (a.in_lds & kVecPostBias) load_param<T, VEC, RAGGED>(a.post_bias, col, in[c], a.param_f32, 0.0f, q);
             if (a.in_lds & kVecGate)                     // (a part's rows share a gate row where the gate is copied)
-                load_param<T, VEC, RAGGED>(a.gate, (long long)(min(first, a.rows - 1) / a.gate_rows) * a.gate_stride + col, in[c], a.param_f32, 1.0f, g);
+                load_param<T, VEC, RAGGED>(a.gate, (long long)(part_first / a.gate_rows) * a.gate_stride + col, in[c], a.param_f32, 1.0f, g);
             if (a.in_lds & kVecGain) store_from_float<float, VEC>(lds + col, w);
             if (a.in_lds & kVecPostGain) store_from_float<float, VEC>(lds_post_gain + col, p);
             if (a.in_lds & kVecPostBias) store_from_float<float, VEC>(lds_post_bias + col, q);
@@ -228,7 +230,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4))) vo
         else load_param<T, VEC, RAGGED>(p, at, count, a.param_f32, other, out);
     };
     // (every group of lanes of a workgroup makes the same number of turns)
-    for (unsigned turn = 0; turn < a.per_part; ++turn) {
+    for (unsigned turn = 0; turn < a.per_group; ++turn) {
         const bool live = first + turn < last;
         if constexpr (SEVERAL) {
             if (!live) break;
@@ -373,22 +375,52 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4))) vo
             }
         }
     }
-    if (!a.vectors || first >= span_end) return;
+    if (!a.vectors) return;
     float* out = a.parts + (size_t)part * __popc(a.vectors) * a.part_stride;
+    if constexpr (SEVERAL) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const unsigned col = (c * lanes + lane) * VEC;
-        if (!in[c]) continue;
-        float* to = out + col;
-        if (a.vectors & kVecGain) store_from_float<float, VEC>(to, sw[c]), to += a.part_stride;
-        if constexpr (BIAS) {
-            if (a.vectors & kVecBias) store_from_float<float, VEC>(to, sz[c]), to += a.part_stride;
+        for (int c = 0; c < C; ++c) {
+            const unsigned col = (c * lanes + lane) * VEC;
+            if (!in[c]) continue;
+            float* to = out + col;
+            if (a.vectors & kVecGain) store_from_float<float, VEC>(to, sw[c]), to += a.part_stride;
+            if constexpr (BIAS) {
+                if (a.vectors & kVecBias) store_from_float<float, VEC>(to, sz[c]), to += a.part_stride;
+            }
+            if (a.vectors & kVecPostGain) store_from_float<float, VEC>(to, sp[c]), to += a.part_stride;
+            if constexpr (BIAS) {
+                if (a.vectors & kVecPostBias) store_from_float<float, VEC>(to, sq[c]), to += a.part_stride;
+            }
+            if (a.vectors & kVecGate) store_from_float<float, VEC>(to, sg[c]);
         }
-        if (a.vectors & kVecPostGain) store_from_float<float, VEC>(to, sp[c]), to += a.part_stride;
+    } else {
+        static_assert(C == 1, "a group of lanes holds one piece a lane");
+        __shared__ float joined[THREADS * VEC];              // [VEC][groups][lanes]
+        auto join = [&](const float (&v)[VEC]) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) joined[i * THREADS + threadIdx.x] = v[i];
+            __syncthreads();
+            if (group == 0 && in[0]) {
+                float o[VEC];
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    o[i] = v[i];
+                    for (unsigned g = lane + lanes; g < THREADS; g += lanes) o[i] += joined[i * THREADS + g];
+                }
+                store_from_float<float, VEC>(out + lane * VEC, o);
+            }
+            out += a.part_stride;
+        };
+        if (a.vectors & kVecGain) join(sw[0]);
         if constexpr (BIAS) {
-            if (a.vectors & kVecPostBias) store_from_float<float, VEC>(to, sq[c]), to += a.part_stride;
+            if (a.vectors & kVecBias) join(sz[0]);
         }
-        if (a.vectors & kVecGate) store_from_float<float, VEC>(to, sg[c]);
+        if (a.vectors & kVecPostGain) join(sp[0]);
+        if constexpr (BIAS) {
+            if (a.vectors & kVecPostBias) join(sq[0]);
+        }
+        if (a.vectors & kVecGate) join(sg[0]);
     }
 }
 
@@ -402,37 +434,46 @@ struct NormMergeArgs {
     long long dgate_stride;
 };
 
-// Sums the parts of a vector (over all of them) or of a gate row (over those of its span): 64 columns a
-// workgroup, 16 wavefronts each adding a run of parts, joined in LDS in that order.
+// Sums the parts of a vector (over all of them) or of a gate row (over those of its span): 16 columns a
+// workgroup, 64 lanes a column each adding every 64th part, joined in LDS in order.
+constexpr int kMergeCols = 16;
+
 template <class T>
 __global__ __launch_bounds__(1024) void block_norm_merge_kernel(NormMergeArgs a) {
-    __shared__ float sh[16][64];
-    const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const unsigned col = blockIdx.x * 64 + lane;
+    __shared__ float sh[64][kMergeCols + 1];
+    const unsigned x = threadIdx.x % kMergeCols, y = threadIdx.x / kMergeCols;
+    const unsigned col = blockIdx.x * kMergeCols + x;
     const unsigned plain = a.per_part_vectors - a.gates;
     const unsigned which = a.first + blockIdx.y;
     const bool gate = which >= plain;
     const unsigned vec = gate ? plain : which, span = gate ? which - plain : 0;
     const unsigned begin = gate ? span * a.parts_per_span : 0;
     const unsigned count = gate ? a.parts_per_span : a.n_parts;
-    const unsigned share = (count + 15) / 16;
-    const unsigned p0 = min(count, wave * share), p1 = min(count, p0 + share);
     const float* from = a.parts + ((size_t)begin * a.per_part_vectors + vec) * a.part_stride + col;
     const size_t step = (size_t)a.per_part_vectors * a.part_stride;
     float acc = 0.0f;
     if (col < a.width)
-        for (unsigned p = p0; p < p1; p += 8) {
+        for (unsigned p = y; p < count; p += 64 * 8) {
             float v[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = p + k < p1 ? from[(p + k) * step] : 0.0f;
+            for (int k = 0; k < 8; ++k) v[k] = p + 64 * k < count ? from[(p + 64 * k) * step] : 0.0f;
 #pragma unroll
             for (int k = 0; k < 8; ++k) acc += v[k];
         }
-    sh[wave][lane] = acc;
+    sh[y][x] = acc;
     __syncthreads();
-    if (wave != 0 || col >= a.width) return;
+    if (y < 8) {
+        acc = 0.0f;
 #pragma unroll
-    for (int w = 1; w < 16; ++w) acc += sh[w][lane];
+        for (int k = 0; k < 8; ++k) acc += sh[y * 8 + k][x];
+    }
+    __syncthreads();
+    if (y < 8) sh[y][x] = acc;
+    __syncthreads();
+    if (y != 0 || col >= a.width) return;
+    acc = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc += sh[k][x];
     if (gate) ((T*)a.dgate)[(long long)span * a.dgate_stride + col] = (T)acc;
     else ((T*)a.out[vec])[col] = (T)acc;
 }

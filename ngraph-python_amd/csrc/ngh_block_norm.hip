@@ -162,7 +162,7 @@ int launch(const ngh_block_norm_spec* s, const NormShape& f, const NormArgs& a, 
 // How the rows of the backward pass are dealt, and where the sums of the parts lie.
 struct GradPlan {
     NormShape shape;
-    unsigned span_rows, spans, parts_per_span, per_part, parts, grid;
+    unsigned span_rows, spans, parts_per_span, per_part, per_group, parts;
     int vectors, count;
     bool gate_whole, bias;
     size_t part_stride, bytes;
@@ -174,28 +174,30 @@ GradPlan plan_grad(const ngh_block_norm_spec* s, int cus) {
     g.vectors = (s->dgain ? kVecGain : 0) | (s->dbias ? kVecBias : 0) | (s->dpost_gain ? kVecPostGain : 0) | (s->dpost_bias ? kVecPostBias : 0);
     g.bias = s->dbias || s->dpost_bias;
     const unsigned rows = (unsigned)s->rows;
-    // 16 wavefronts a compute unit (what the registers allow), but at least 8 rows a part, for a part's sums are
-    // written in fp32 and read once more; fewer, down to 2, where else compute units would have no part.
-    const unsigned groups = g.shape.rows_a_workgroup();                                  // parts a workgroup holds
-    const unsigned want = std::max(1u, 1024u / g.shape.threads()) * cus * groups;
-    const unsigned least = std::min(8u, std::max(2u, rows / (2u * cus * groups)));
+    // 16 wavefronts a compute unit (what the registers allow; a workgroup of 5 takes the room of 8), but at least
+    // 8 rows a part, for a part's sums are written in fp32 and read once more; fewer, down to 2, where else
+    // compute units would have no part.
+    const unsigned groups = g.shape.rows_a_workgroup();
+    const unsigned want = 1024u / ((g.shape.threads() + 255u) / 256u * 256u) * cus;
+    const unsigned least = std::min(8u, std::max(2u, rows / (2u * cus)));
     g.per_part = std::max(least, (rows + want - 1) / want);
+    g.per_group = (g.per_part + groups - 1) / groups;
     const unsigned gate_rows = (unsigned)std::max<int64_t>(1, s->gate_rows);
-    g.gate_whole = !s->dgate || gate_rows < 2 * g.per_part;
+    g.gate_whole = !s->dgate || gate_rows < 2 * g.per_group;
     g.span_rows = g.gate_whole ? std::max(1u, rows) : gate_rows;
     if (!g.gate_whole) {
         // the rows of a gate row are shared by as many parts as they fill
         g.vectors |= kVecGate;
-        const unsigned parts = gate_rows / g.per_part;
-        g.per_part = (gate_rows + parts - 1) / parts;
+        const unsigned parts = std::max(1u, gate_rows / g.per_part);
+        g.per_group = ((gate_rows + parts - 1) / parts + groups - 1) / groups;
     } else if (s->dgate) {
-        g.per_part = std::max(1u, g.per_part / gate_rows) * gate_rows;                   // (whole gate rows)
+        g.per_group = std::max(1u, g.per_group / gate_rows) * gate_rows;                 // (whole gate rows)
     }
+    g.per_part = g.per_group * groups;
     g.count = __builtin_popcount((unsigned)g.vectors);
     g.spans = g.gate_whole ? 1 : rows / g.span_rows;
     g.parts_per_span = (g.span_rows + g.per_part - 1) / g.per_part;
     g.parts = g.spans * g.parts_per_span;
-    g.grid = (g.parts + groups - 1) / groups;
     g.part_stride = ((size_t)s->width + 7) / 8 * 8;
     g.bytes = (size_t)g.parts * g.count * g.part_stride * 4;
     return g;
@@ -205,7 +207,7 @@ template <class T>
 int launch_merge(NormMergeArgs m, unsigned spans, hipStream_t stream) {
     const unsigned sums = m.per_part_vectors - m.gates + (m.gates ? spans : 0);
     for (m.first = 0; m.first < sums; m.first += 65535u) {
-        hipLaunchKernelGGL(block_norm_merge_kernel<T>, dim3((m.width + 63) / 64, std::min(65535u, sums - m.first)), dim3(1024), 0, stream, m);
+        hipLaunchKernelGGL(block_norm_merge_kernel<T>, dim3((m.width + kMergeCols - 1) / kMergeCols, std::min(65535u, sums - m.first)), dim3(1024), 0, stream, m);
         NGH_HIP_TRY(hipGetLastError());
     }
     return NGH_OK;
@@ -264,6 +266,7 @@ int ngh_block_norm_grad(ngh_context* ctx, const ngh_block_norm_spec* spec) {
     a.span_rows = g.span_rows;
     a.parts_per_span = g.parts_per_span;
     a.per_part = g.per_part;
+    a.per_group = g.per_group;
     a.vectors = g.vectors;
     a.gate_whole = g.gate_whole;
     // Vectors copied to LDS, as far as 48 KiB go (64 KiB a workgroup without further ado, the reductions' words
@@ -271,7 +274,7 @@ int ngh_block_norm_grad(ngh_context* ctx, const ngh_block_norm_spec* spec) {
     a.lds_stride = (a.width + 7) / 8 * 8;
     const int wanted[4][2] = {{kVecGain, spec->gain != nullptr},
                               {kVecPostGain, spec->post_gain != nullptr},
-                              {kVecGate, spec->gate != nullptr && (spec->gate_rows == spec->rows || (!g.gate_whole && g.shape.rows_a_workgroup() == 1))},
+                              {kVecGate, spec->gate != nullptr && (spec->gate_rows == spec->rows || !g.gate_whole)},
                               {kVecPostBias, spec->post_bias != nullptr}};
     size_t room = 48u << 10;
     for (const auto& w : wanted)
@@ -280,7 +283,7 @@ int ngh_block_norm_grad(ngh_context* ctx, const ngh_block_norm_spec* spec) {
             room -= a.lds_stride * 4;
         }
     if (spec->rows) {
-        const int lrc = launch(spec, g.shape, a, g.bias ? kNormBackwardBias : kNormBackward, g.grid, c.stream);
+        const int lrc = launch(spec, g.shape, a, g.bias ? kNormBackwardBias : kNormBackward, g.parts, c.stream);
         if (lrc != NGH_OK) return lrc;
     }
     if (!g.vectors) return NGH_OK;
