@@ -4,8 +4,7 @@
 // chunks it takes; a chunk is kChunk elements, so that one large matrix and a hundred short vectors
 // keep the chip equally busy.  With fp32 states and gradients an element moves 28 bytes (p, m, v in
 // and out, g in), with 8-bit states and bf16 gradients 14: bound by memory either way, though 8-bit
-// states take some 150 vector instructions an element (two quotients and three roots, correctly
-// rounded, for the codes alone).
+// states need two quotients and three roots, correctly rounded, for the codes of an element (four_codes).
 //
 // 8-bit states.  256 consecutive elements share a scale.  A wavefront holds a block, 4 consecutive
 // elements a lane: the largest |moment| is a butterfly over the lanes, on the bit patterns as unsigned
@@ -68,12 +67,6 @@ struct StepArgs {
     int copy_dtype;
 };
 
-__device__ __forceinline__ unsigned wave_max(unsigned x) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) x = max(x, (unsigned)__shfl_xor((int)x, m, 64));
-    return x;
-}
-
 // The scale of a block from the bit patterns of its magnitudes.
 __device__ __forceinline__ float scale_of(unsigned bits) {
     const unsigned top = wave_max(bits);
@@ -99,6 +92,32 @@ __device__ __forceinline__ float first_value(int q, float s) {
 __device__ __forceinline__ float second_value(int q, float s) {
     const float t = (float)q * (float)(1.0 / 255.0);
     return ((t * t) * (t * t)) * s;
+}
+
+// The codes of a lane's four moments of either kind.  They are decided by the correctly rounded quotient and
+// roots above, which take some 90 instructions an element for both; here approximate ones (v_rcp, v_sqrt: 1 ulp)
+// place the root within 7.5 * 2^-24 * 255 = 1.2e-4 steps of the exact chain's, so that only a root that
+// lies within 2^-12 of the border of two codes has to be worked out exactly, for the whole wavefront then (one
+// in eight blocks).  Scales too small for an approximate reciprocal take that way too.
+template <bool SECOND>
+__device__ __forceinline__ unsigned four_codes(const float (&x)[kPer], float s) {
+    unsigned w = 0;
+    bool close = !(s >= 0x1p-100f);
+    const float r = __builtin_amdgcn_rcpf(s);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const float root = __builtin_amdgcn_sqrtf(fabsf(x[j]) * r);
+        const float y = SECOND ? __builtin_amdgcn_sqrtf(root) * 255.0f : copysignf(root * 127.0f, x[j]);
+        const float q = rintf(y);
+        close = close || !(fabsf(y - q) <= 0.5f - 0x1p-12f);
+        w |= ((unsigned)(int)q & 255u) << (8 * j);
+    }
+    if (__any(close)) {
+        w = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) w |= ((unsigned)(SECOND ? second_code(x[j], s) : first_code(x[j], s)) & 255u) << (8 * j);
+    }
+    return w;
 }
 
 template <class T>
@@ -187,8 +206,12 @@ __global__ __launch_bounds__(kAdamBlock) void adamw_kernel(StepArgs a) {
             const float gj = g[t][j] * gs;
             m[t][j] = m[t][j] * a.beta1 + gj * a.rest1;
             v[t][j] = v[t][j] * a.beta2 + (gj * gj) * a.rest2;
-            const float root = sqrtf(v[t][j]) * k.root2 + a.eps;
-            p[t][j] = p[t][j] * keep - m[t][j] / root * k.a;
+            // (the step itself to a few ulp: approximate root and reciprocal, unless eps is so small that
+            // what they do to the smallest numbers would show)
+            float step;
+            if (a.eps >= 1e-12f) step = m[t][j] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[t][j]) * k.root2 + a.eps) * k.a;
+            else step = m[t][j] / (sqrtf(v[t][j]) * k.root2 + a.eps) * k.a;
+            p[t][j] = p[t][j] * keep - step;
             if (BITS == 8 && j < count) {
                 mtop = max(mtop, __float_as_uint(m[t][j]) & 0x7fffffffu);
                 vtop = max(vtop, __float_as_uint(v[t][j]) & 0x7fffffffu);
@@ -205,14 +228,8 @@ __global__ __launch_bounds__(kAdamBlock) void adamw_kernel(StepArgs a) {
             store_four((float*)r.v, at, count, whole, v[t]);
         } else {
             const float s1 = scale_of(mtop), s2 = scale_of(vtop);
-            unsigned w1 = 0, w2 = 0;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                w1 |= ((unsigned)first_code(m[t][j], s1) & 255u) << (8 * j);
-                w2 |= (unsigned)second_code(v[t][j], s2) << (8 * j);
-            }
-            store_codes((unsigned char*)r.m, at, count, whole, w1);
-            store_codes((unsigned char*)r.v, at, count, whole, w2);
+            store_codes((unsigned char*)r.m, at, count, whole, four_codes<false>(m[t], s1));
+            store_codes((unsigned char*)r.v, at, count, whole, four_codes<true>(v[t], s2));
             if ((threadIdx.x & 63) == 0 && count > 0) {
                 r.m_scale[at / NGH_ADAMW_BLOCK] = s1;
                 r.v_scale[at / NGH_ADAMW_BLOCK] = s2;

@@ -93,27 +93,39 @@ __device__ __forceinline__ int piece_count(unsigned col, unsigned width) {
     else return col < width ? V : 0;
 }
 
-// x plus the x of the lane's partner at distance 1, 2, 4, 8, 16 or 32, where the lanes at smaller
-// distances hold the same sum already: one instruction each within 16 lanes (the partner of a mirror is
-// not the lane at that distance but one with the same sum), two beyond.
+// The x of the lane's partner at distance 1, 2, 4, 8, 16 or 32 for reductions in which the lanes at smaller
+// distances hold the same value already: one instruction within 16 lanes, mostly part of the one that
+// uses it (the partner of a mirror is not the lane at that distance but one with the same value), and
+// one for a pair of values beyond.
 template <int CTRL>
-__device__ __forceinline__ float add_dpp(float x) {
-    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+__device__ __forceinline__ unsigned dpp(unsigned x) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+}
+
+template <int DISTANCE, class F>
+__device__ __forceinline__ unsigned with_partner(unsigned x, F f) {
+    if constexpr (DISTANCE == 1) return f(x, dpp<0xB1>(x));          // quad_perm 1,0,3,2
+    else if constexpr (DISTANCE == 2) return f(x, dpp<0x4E>(x));     // quad_perm 2,3,0,1
+    else if constexpr (DISTANCE == 4) return f(x, dpp<0x141>(x));    // row_half_mirror
+    else if constexpr (DISTANCE == 8) return f(x, dpp<0x140>(x));    // row_mirror
+    else if constexpr (DISTANCE == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        return f(r[0], r[1]);
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        return f(r[0], r[1]);
+    }
 }
 
 template <int DISTANCE>
 __device__ __forceinline__ float add_partner(float x) {
-    if constexpr (DISTANCE == 1) return add_dpp<0xB1>(x);          // quad_perm 1,0,3,2
-    else if constexpr (DISTANCE == 2) return add_dpp<0x4E>(x);     // quad_perm 2,3,0,1
-    else if constexpr (DISTANCE == 4) return add_dpp<0x141>(x);    // row_half_mirror
-    else if constexpr (DISTANCE == 8) return add_dpp<0x140>(x);    // row_mirror
-    else if constexpr (DISTANCE == 16) {
-        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    } else {
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
+    return __uint_as_float(with_partner<DISTANCE>(
+        __float_as_uint(x), [](unsigned a, unsigned b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+
+__device__ __forceinline__ unsigned wave_max(unsigned x) {
+    const auto f = [](unsigned a, unsigned b) { return max(a, b); };
+    return with_partner<32>(with_partner<16>(with_partner<8>(with_partner<4>(with_partner<2>(with_partner<1>(x, f), f), f), f), f), f);
 }
 
 // The sums over the lanes of a row of up to kRowSumsMax values.  SEVERAL: the row has several wavefronts

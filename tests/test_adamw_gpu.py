@@ -1,8 +1,11 @@
 """ngh_adamw_* against NumPy.
 
 The moments and the 8-bit codes are defined by fp32 operations in a fixed order, which NumPy's
-correctly rounded fp32 repeats: they are compared bit for bit.  The update is compared with float64:
-it has 10 roundings of 2^-24 relative to the parameter and to the step, then one to the type.
+correctly rounded fp32 repeats: they are compared bit for bit.  The update is compared with float64.
+In units of u = 2^-24 its step is off by 2 (root, 1 ulp) + 2 (times a factor that is rounded itself) + 1
+(plus eps) + 2 (reciprocal, 1 ulp) + 1 (times m) + 2 (times the rounded rate) = 10 of its size, the parameter
+by 2 (times a rounded factor) + 1 (the difference) of its own, the difference by 1 of the step: 11 and
+3, 12 and 4 with the second order; then one rounding to the type.
 """
 import numpy as np
 import pytest
@@ -48,7 +51,7 @@ def updated(p, m, v, decay, t, k):
     m, v, p = m.astype(f64), v.astype(f64), p.astype(f64)
     step = k["lr"] / (1 - k["beta1"] ** t) * m / (np.sqrt(v) / np.sqrt(1 - k["beta2"] ** t) + k["eps"])
     want = p * (1 - k["lr"] * decay) - step
-    return want, EPS * (4 * np.abs(p) + 10 * np.abs(step))
+    return want, EPS * (4 * np.abs(p) + 12 * np.abs(step))
 
 
 class Model(object):
@@ -157,6 +160,31 @@ def test_hundreds_of_tensors(hip_runtime, bits):
         model = Model(pool, hip_runtime, [int(s) for s in sizes], ("f32", "bf16"), bits)
         hip_runtime.adamw_step(model.plan, 7, grad_scale=0.25, **HYPER)
         model.check_step(7, 0.25)
+        model.free()
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-13, 1e-12, 1e-3])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_small_second_moments_and_any_eps(hip_runtime, bits, eps):
+    """Gradients down to where their squares leave the normal numbers."""
+    with Pool(hip_runtime) as pool:
+        model = Model(pool, hip_runtime, [4000], ("f32", "f32"), bits)
+        t = model.tensors[0]
+        rs = np.random.RandomState(4)
+        t["g"] = (rs.normal(0, 1, 4000) * 10.0 ** -(4 + np.arange(4000) // 256)).astype(f32)
+        t["g"][t["g"] == 0] = f32(1e-10)
+        hip_runtime.memcpy_h2d(t["dev_g"].ptr, t["g"])
+        if bits == 32:
+            for name in ("m", "v"):
+                t[name] = (t["g"] * t["g"] if name == "v" else t["g"]).astype(f32)
+                hip_runtime.memcpy_h2d(t["dev_" + name].ptr, t[name])
+            hyper = dict(HYPER, eps=eps)
+            hip_runtime.adamw_step(model.plan, 3, **hyper)
+            model.check_step(3, hyper=hyper)
+        else:
+            hyper = dict(HYPER, eps=max(eps, 1e-13))          # (8 bits hold moments that are 0)
+            hip_runtime.adamw_step(model.plan, 3, **hyper)
+            model.check_step(3, hyper=hyper)
         model.free()
 
 
