@@ -1,8 +1,7 @@
 // AdamW over many tensors at once (ngh_adamw_* in ngraph_hip.h): one launch for all of them.
 //
 // The plan holds a record for each tensor and, for each workgroup, which tensor and which of its
-// chunks it takes; a chunk is kChunk elements, so that one large matrix and a hundred short vectors
-// keep the chip equally busy.  With fp32 states and gradients an element moves 28 bytes (p, m, v in
+// chunks it takes, so that one large matrix and a hundred short vectors keep the chip equally busy.  With fp32 states and gradients an element moves 28 bytes (p, m, v in
 // and out, g in), with 8-bit states and bf16 gradients 14: bound by memory either way, though 8-bit
 // states need two quotients and three roots, correctly rounded, for the codes of an element (four_codes).
 //
@@ -31,8 +30,9 @@ namespace {
 
 constexpr int kAdamBlock = 256;
 constexpr int kPer = 4;                        // elements a lane takes at a time: a wavefront takes NGH_ADAMW_BLOCK
-constexpr int kTurns = 4;
-constexpr int kChunk = kAdamBlock * kPer * kTurns;
+// A workgroup takes a chunk of TURNS * 1024 elements of one tensor, a lane's TURNS pieces of it in flight together.
+constexpr int kPiece = kAdamBlock * kPer;
+constexpr int kTurnsMany = 4, kTurnsFew = 1;
 static_assert(64 * kPer == NGH_ADAMW_BLOCK, "a wavefront holds one block of 8-bit states");
 
 struct Record {
@@ -160,20 +160,20 @@ __device__ __forceinline__ void store_codes(unsigned char* p, long long at, int 
         if (j < count) p[at + j] = (unsigned char)(w >> (8 * j));
 }
 
-template <class P, class G, int BITS>
+template <class P, class G, int BITS, int TURNS>
 __global__ __launch_bounds__(kAdamBlock) void adamw_kernel(StepArgs a) {
     const Job job = a.jobs[blockIdx.x];
     const Record r = a.records[job.tensor];
     const Scalars k = a.dev ? *a.dev : a.by_value;
     const float gs = a.dev_grad_scale ? a.grad_scale * *a.dev_grad_scale : a.grad_scale;
     const float keep = 1.0f - k.lr * r.weight_decay;
-    const long long first = (long long)job.chunk * kChunk + threadIdx.x * kPer;
-    float p[kTurns][kPer], g[kTurns][kPer], m[kTurns][kPer], v[kTurns][kPer];
-    unsigned mq[kTurns], vq[kTurns];
-    float ms[kTurns], vs[kTurns];
+    const long long first = (long long)job.chunk * (TURNS * kPiece) + threadIdx.x * kPer;
+    float p[TURNS][kPer], g[TURNS][kPer], m[TURNS][kPer], v[TURNS][kPer];
+    unsigned mq[TURNS], vq[TURNS];
+    float ms[TURNS], vs[TURNS];
 #pragma unroll
-    for (int t = 0; t < kTurns; ++t) {
-        const long long at = first + t * (kAdamBlock * kPer);
+    for (int t = 0; t < TURNS; ++t) {
+        const long long at = first + t * kPiece;
         const int count = (int)max(0ll, min((long long)kPer, r.n - at));
         const bool whole = r.aligned && count == kPer;
         load_four((const P*)r.param, at, count, whole, p[t]);
@@ -189,8 +189,8 @@ __global__ __launch_bounds__(kAdamBlock) void adamw_kernel(StepArgs a) {
         }
     }
 #pragma unroll
-    for (int t = 0; t < kTurns; ++t) {
-        const long long at = first + t * (kAdamBlock * kPer);
+    for (int t = 0; t < TURNS; ++t) {
+        const long long at = first + t * kPiece;
         const int count = (int)max(0ll, min((long long)kPer, r.n - at));
         const bool whole = r.aligned && count == kPer;
         if constexpr (BITS == 8) {
@@ -301,6 +301,7 @@ struct ngh_adamw_plan {
     int device = 0;
     int param_dtype = 0, grad_dtype = 0, copy_dtype = -1, bits = 32;
     unsigned jobs = 0;
+    int turns = kTurnsMany;
     void* memory = nullptr;            // scalars, records, jobs
     const Record* dev_records = nullptr;
     const Job* dev_jobs = nullptr;
@@ -311,7 +312,7 @@ namespace ngh {
 namespace {
 
 // Checks the tensors and works out the plan's records and jobs; touches no device.
-int lay_out(const ngh_adamw_tensor* tensors, int32_t n_tensors, const ngh_adamw_plan& plan, std::vector<Record>& records, std::vector<Job>& jobs) {
+int lay_out(const ngh_adamw_tensor* tensors, int32_t n_tensors, int cus, ngh_adamw_plan& plan, std::vector<Record>& records, std::vector<Job>& jobs) {
     if (n_tensors < 0 || (n_tensors > 0 && !tensors)) return report(NGH_E_INVALID, "ngh_adamw: %d tensors", n_tensors);
     if (!size_of(plan.param_dtype) || !size_of(plan.grad_dtype) || (plan.copy_dtype != -1 && !size_of(plan.copy_dtype)))
         return report(NGH_E_INVALID, "ngh_adamw: dtypes %d, %d, %d (NGH_F32, NGH_F16, NGH_BF16; no copy: -1)", plan.param_dtype, plan.grad_dtype,
@@ -359,10 +360,16 @@ int lay_out(const ngh_adamw_tensor* tensors, int32_t n_tensors, const ngh_adamw_
             span(t.m_scale, blocks * 4, true);
             span(t.v_scale, blocks * 4, true);
         }
-        const long long chunks = (t.n + kChunk - 1) / kChunk;
-        if (chunks + (long long)jobs.size() >= (1LL << 31)) return report(NGH_E_UNSUPPORTED, "ngh_adamw: too many elements for one plan");
-        for (long long c = 0; c < chunks; ++c) jobs.push_back(Job{i, (int)c});
     }
+    // Chunks of 4096 elements, of 1024 where else compute units would have fewer than four workgroups (1.3 M
+    // parameters in 69 tensors: 8.4 -> 7.6 us, with 8-bit states 10.2 -> 7.5; 82 thousand 5.7 -> 3.5)
+    long long pieces = 0;
+    for (int i = 0; i < n_tensors; ++i) pieces += (tensors[i].n + kPiece - 1) / kPiece;
+    plan.turns = pieces >= 4ll * kTurnsMany * cus ? kTurnsMany : kTurnsFew;
+    const long long chunk = (long long)plan.turns * kPiece;
+    if (pieces >= (1LL << 31)) return report(NGH_E_UNSUPPORTED, "ngh_adamw: too many elements for one plan");
+    for (int i = 0; i < n_tensors; ++i)
+        for (long long c = 0; c * chunk < tensors[i].n; ++c) jobs.push_back(Job{i, (int)c});
     // nothing that is written may be anything else of the plan
     std::sort(spans.begin(), spans.end(), [](const Span& x, const Span& y) { return x.begin < y.begin; });
     uintptr_t end = 0, end_written = 0;
@@ -380,7 +387,7 @@ int lay_out(const ngh_adamw_tensor* tensors, int32_t n_tensors, const ngh_adamw_
 int make_plan(ngh_context* ctx, const ngh_adamw_tensor* tensors, int32_t n_tensors, ngh_adamw_plan& plan) {
     std::vector<Record> records;
     std::vector<Job> jobs;
-    const int rc = lay_out(tensors, n_tensors, plan, records, jobs);
+    const int rc = lay_out(tensors, n_tensors, view_of(ctx).cus, plan, records, jobs);
     if (rc != NGH_OK) return rc;
     plan.jobs = (unsigned)jobs.size();
     if (jobs.empty()) return NGH_OK;
@@ -399,10 +406,16 @@ int make_plan(ngh_context* ctx, const ngh_adamw_tensor* tensors, int32_t n_tenso
     return NGH_OK;
 }
 
+template <class P, class G, int BITS>
+void launch_step(const ngh_adamw_plan& plan, const StepArgs& a, hipStream_t stream) {
+    if (plan.turns == kTurnsMany) hipLaunchKernelGGL((adamw_kernel<P, G, BITS, kTurnsMany>), dim3(plan.jobs), dim3(kAdamBlock), 0, stream, a);
+    else hipLaunchKernelGGL((adamw_kernel<P, G, BITS, kTurnsFew>), dim3(plan.jobs), dim3(kAdamBlock), 0, stream, a);
+}
+
 template <class P, class G>
 void launch_step(const ngh_adamw_plan& plan, const StepArgs& a, hipStream_t stream) {
-    if (plan.bits == 8) hipLaunchKernelGGL((adamw_kernel<P, G, 8>), dim3(plan.jobs), dim3(kAdamBlock), 0, stream, a);
-    else hipLaunchKernelGGL((adamw_kernel<P, G, 32>), dim3(plan.jobs), dim3(kAdamBlock), 0, stream, a);
+    if (plan.bits == 8) launch_step<P, G, 8>(plan, a, stream);
+    else launch_step<P, G, 32>(plan, a, stream);
 }
 
 template <class P>
@@ -441,7 +454,7 @@ int ngh_validate_adamw(const ngh_adamw_tensor* tensors, int32_t n_tensors, int32
     try {
         std::vector<Record> records;
         std::vector<Job> jobs;
-        return lay_out(tensors, n_tensors, plan, records, jobs);
+        return lay_out(tensors, n_tensors, 256, plan, records, jobs);
     } catch (const std::exception&) {
         return report(NGH_E_NOMEM, "ngh_validate_adamw: out of host memory");
     }
