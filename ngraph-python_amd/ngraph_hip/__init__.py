@@ -32,4 +32,20 @@ def contiguous(x):
     return _ContiguousOp(x)
 
 
+def embedding(table, tokens, scale=1.0, pad_idx=None):
+    """scale * table[tokens, :] for int32 tokens, zeros for pad_idx and tokens outside the table
+    (op_graph/lookuptable.py:20-115 is the reference's lookup); differentiable in the table."""
+    from ngraph_hip.transformers import hiprows
+    return hiprows.embedding(table, tokens, scale, pad_idx)
+
+
+def block_norm(x, b=None, gain=None, bias=None, post_gain=None, post_bias=None, gate=None, kind="rms", post_norm=None, residual_scale=1.0,
+               eps=1e-5):
+    """(y, h): the stream h = residual_scale * x + gate * (N(b) * post_gain + post_bias) after a block with output
+    b, and the next block's input y = N(h) * gain + bias; N the rms or layer norm over the last axis
+    (transformers/hiprows.py)."""
+    from ngraph_hip.transformers import hiprows
+    return hiprows.block_norm(x, b, gain, bias, post_gain, post_bias, gate, kind, post_norm, residual_scale, eps)
+
+
 __version__ = "0.1.0"

@@ -256,6 +256,48 @@ class Adam(Optimizer):
         return updates, m, v
 
 
+class AdamW(Optimizer):
+    """Adam with decoupled weight decay, every variable updated in one launch, moments in fp32 or 8 bits:
+
+        p = p (1 - lr weight_decay) - lr / (1 - beta_1^t) m / (sqrt(v) / sqrt(1 - beta_2^t) + epsilon)
+
+    The reference's Adam (frontends/neon/optimizer.py:446-470, `Adam` above) is a kernel for each
+    variable, keeps epsilon outside the bias correction and decays nothing.  learning_rate may be a scalar
+    op.  `decayed` chooses the variables that decay (default: those of two axes or more, which leaves
+    gains and biases out).  `minimize` returns an op whose AdamWOp is kept as `update`: its `step`, `m`
+    and `v` are persistent tensors."""
+
+    def __init__(self, learning_rate=1e-3, beta_1=0.9, beta_2=0.999, epsilon=1e-8, weight_decay=0.01, state_bits=32, decayed=None,
+                 **clipping):
+        self._set_clipping(**clipping)
+        self.lrate, self.beta_1, self.beta_2, self.epsilon = learning_rate, beta_1, beta_2, epsilon
+        self.weight_decay, self.state_bits = weight_decay, state_bits
+        self.decayed = decayed if decayed is not None else lambda variable: len(variable.axes) >= 2
+        self.update = None
+
+    def minimize(self, cost_func, variables=None):
+        from ngraph_hip.transformers.hiprows import AdamWOp
+        batch_cost = ng.sum(cost_func, out_axes=())
+        batch_axis = cost_func.axes.batch_axis()
+        share = 1.0 if batch_axis is None else 1.0 / batch_axis.length
+        if variables is None:
+            variables = trainable_variables(batch_cost)
+        grads = [ng.deriv(batch_cost, v) for v in variables]
+        factor = None
+        if self.gradient_clip_norm is not None:
+            factor = clip_gradient_norm([g * share for g in grads], self.gradient_clip_norm)
+        if self.gradient_clip_value is not None:
+            # (the values that are clipped are those of the mean gradient)
+            grads = [clip_gradient_value(g * share, self.gradient_clip_value) for g in grads]
+            share = 1.0
+        self.update = AdamWOp(variables, grads, self.lrate, self.beta_1, self.beta_2, self.epsilon,
+                              [self.weight_decay if self.decayed(v) else 0.0 for v in variables], self.state_bits, share, factor)
+        steps = [self.update]
+        if self.weight_clip_value is not None:
+            steps += [ng.assign(v, clip_weight_value(v, self.weight_clip_value)) for v in variables]
+        return ng.sequential(steps + [batch_cost])
+
+
 class GradientDescentMomentum(Optimizer):
     """SGD with momentum, weight decay, optional Nesterov step and the Kahan-compensated
     parameter update of frontends/neon/optimizer.py:285-310."""

@@ -16,7 +16,7 @@ registry through its metaclass (base.py:265-279) and are made by its
 package is imported before `register` is called, so this module imports anywhere.
 
 How: the lowering (`ngraph_hip/transformers/hiptransform.py` and the modules it is made of --
-`hipdevice`, `hiplowering`, `hipmoments`, `hipchains`, `hipplanner` --, `flexhiptransform.py`,
+`hipdevice`, `hiplowering`, `hipmoments`, `hiprows`, `hipchains`, `hipplanner` --, `flexhiptransform.py`,
 `passes/hippasses.py`) reaches the graph package only through `import` statements naming
 `ngraph_hip.op_graph...`, `ngraph_hip.transformers.base` and
 `ngraph_hip.transformers.passes.passes` -- the modules this repository carries as stand-ins for
@@ -151,7 +151,7 @@ SUBSTITUTED = {
 #: modules executed again per package, in dependency order
 REBOUND = ("ngraph_hip.transformers.passes.hippasses", "ngraph_hip.transformers.hipdevice",
            "ngraph_hip.transformers.hiplowering", "ngraph_hip.transformers.hipmoments",
-           "ngraph_hip.transformers.hipchains", "ngraph_hip.transformers.hipplanner",
+           "ngraph_hip.transformers.hiprows", "ngraph_hip.transformers.hipchains", "ngraph_hip.transformers.hipplanner",
            "ngraph_hip.transformers.hiptransform", "ngraph_hip.transformers.flexhiptransform")
 
 _bound = {}
@@ -164,6 +164,7 @@ class Bound(object):
         self.package, self.modules = package, modules
         self.hiptransform = modules["ngraph_hip.transformers.hiptransform"]
         self.flexhiptransform = modules["ngraph_hip.transformers.flexhiptransform"]
+        self.hiprows = modules["ngraph_hip.transformers.hiprows"]       # embedding, block_norm, AdamWOp for the package's graphs
         self.HipTransformer = self.hiptransform.HipTransformer
         self.FlexHipTransformer = self.flexhiptransform.FlexHipTransformer
 

@@ -346,11 +346,14 @@ class HipRuntime(row_ops.OperatorCalls):
         _check(self.lib, self.lib.ngh_init(int(device_id), ctypes.byref(ctx)))
         self.ctx = ctx
         self._allocs = set()
+        self._adamw_plans = []
         self.program_libraries = []        # what this context asked the library to load
 
     # -- lifetime --------------------------------------------------------
     def close(self):
         if getattr(self, "ctx", None):
+            for plan in list(self._adamw_plans):
+                self.adamw_plan_free(plan)
             for ptr in list(self._allocs):
                 self.lib.ngh_free(self.ctx, ctypes.c_void_p(ptr))
             self._allocs.clear()
@@ -593,11 +596,16 @@ class HipRuntime(row_ops.OperatorCalls):
         return ms.value
 
 
-class DryRunRuntime(object):
+class DryRunRuntime(row_ops.DryRunOperatorCalls, row_ops.OperatorCalls):
     """Stands in for HipRuntime where no device exists: hands out fake, aligned device
     addresses and records launches.  It lets the host-side lowering (graph -> kernel specs)
     run and be validated by the library on a machine without a GPU; it computes nothing,
     and reading results through it raises."""
+
+    abi_version = NGH_ABI_VERSION
+
+    def _check(self, rc):
+        _check(self.lib, rc)
 
     def __init__(self):
         self.lib = load_library()

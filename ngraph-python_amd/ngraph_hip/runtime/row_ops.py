@@ -79,10 +79,40 @@ def adamw_tensors(rows):
 
 
 class AdamWPlan(object):
-    """Handle of ngh_adamw_plan_create; freed by `free()` or with its runtime."""
+    """Handle of ngh_adamw_plan_create; freed by `adamw_plan_free` or with its runtime."""
 
     def __init__(self, handle, n_tensors, state_bits):
         self.handle, self.n_tensors, self.state_bits = handle, n_tensors, state_bits
+
+
+class DryRunOperatorCalls(object):
+    """The same calls where no device exists: specs are checked by the library and recorded."""
+
+    def embedding(self, spec):
+        self._check(self.lib.ngh_validate_embedding(ctypes.byref(spec), 0))
+        self.launched.append(spec)
+
+    def embedding_grad(self, spec):
+        self._check(self.lib.ngh_validate_embedding(ctypes.byref(spec), 1))
+        self.launched.append(spec)
+
+    def block_norm(self, spec):
+        self._check(self.lib.ngh_validate_block_norm(ctypes.byref(spec), 0))
+        self.launched.append(spec)
+
+    def block_norm_grad(self, spec):
+        self._check(self.lib.ngh_validate_block_norm(ctypes.byref(spec), 1))
+        self.launched.append(spec)
+
+    def adamw_plan(self, tensors, param_dtype=0, grad_dtype=0, copy_dtype=-1, state_bits=32):
+        self._check(self.lib.ngh_validate_adamw(adamw_tensors(tensors), len(tensors), param_dtype, grad_dtype, copy_dtype, state_bits))
+        return AdamWPlan(None, len(tensors), state_bits)
+
+    def adamw_step(self, plan, **hyper):
+        self.launched.append(("adamw", plan, hyper))
+
+    def adamw_plan_free(self, plan):
+        pass
 
 
 class OperatorCalls(object):
@@ -168,7 +198,9 @@ class OperatorCalls(object):
         handle = _vp()
         self._check(self.lib.ngh_adamw_plan_create(self.ctx, adamw_tensors(tensors), len(tensors), param_dtype, grad_dtype,
                                                    copy_dtype, state_bits, ctypes.byref(handle)))
-        return AdamWPlan(handle, len(tensors), state_bits)
+        plan = AdamWPlan(handle, len(tensors), state_bits)
+        self._adamw_plans.append(plan)
+        return plan
 
     def adamw_step(self, plan, step=0, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, dev_step=None, dev_lr=None,
                    dev_grad_scale=None):
@@ -177,6 +209,8 @@ class OperatorCalls(object):
         self._check(self.lib.ngh_adamw_step(self.ctx, plan.handle, ctypes.byref(h)))
 
     def adamw_plan_free(self, plan):
+        if plan in self._adamw_plans:
+            self._adamw_plans.remove(plan)
         handle, plan.handle = plan.handle, None
         self._check(self.lib.ngh_adamw_plan_free(self.ctx, handle))
 

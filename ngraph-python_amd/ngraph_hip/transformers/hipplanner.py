@@ -312,6 +312,8 @@ class FusionPlanner(object):
                 if isinstance(o, (og.AssignOp, og.Fill)) and \
                         _td(o.args[0].forwarded).base in bases:
                     return True
+                if any(t.tensor_description().base in bases for t in getattr(o, "written_tensors", ())):
+                    return True
         return False
 
 

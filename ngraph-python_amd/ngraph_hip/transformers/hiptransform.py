@@ -18,7 +18,8 @@ Plays the part of ngraph/transformers/gputransform.py for this path:
   (gputransform.py:525-909).
 
 The parts live in modules of their own: `hipdevice` (device memory, host I/O), `hiplowering`
-(op names, operands, programs, `FusedKernel`), `hipmoments` (one-pass statistics), `hipchains`
+(op names, operands, programs, `FusedKernel`), `hipmoments` (one-pass statistics), `hiprows` (embedding,
+block norms, AdamW), `hipchains`
 (several kernels as the stages of one launch), `hipplanner` (which ops share a kernel); this
 module holds the executor loop and the transformer, and re-exports the names others import.
 
@@ -43,6 +44,7 @@ from ngraph_hip.transformers.hipdevice import HipDeviceBufferStorage, HipDeviceT
 from ngraph_hip.transformers.hiplowering import (FusedKernel, CopyKernel, HipKernel, kernel_op_name,  # noqa: F401
                                                  is_fusable, iteration_axes, og_unsupported)
 from ngraph_hip.transformers.hipmoments import MomentsOp, MomentsFusionPass, MomentsKernel, moments_layout  # noqa: F401
+from ngraph_hip.transformers.hiprows import row_kernel
 from ngraph_hip.transformers.hipchains import ChainKernel, KernelRun  # noqa: F401
 from ngraph_hip.transformers.hipplanner import FusionPlanner
 
@@ -400,7 +402,10 @@ class HipTransformer(ComputationGraphTransformer):
                 elif isinstance(op, MomentsOp):
                     group.kernels.append(MomentsKernel(self, op))
                 else:
-                    raise ValueError("Unhandled op: {}".format(op))
+                    kernel = row_kernel(self, op)
+                    if kernel is None:
+                        raise ValueError("Unhandled op: {}".format(op))
+                    group.kernels.append(kernel)
         if self.chain_kernels and self.fusion:
             group.kernels = self._chained(group.kernels)
         self.kernel_groups[computation] = group
