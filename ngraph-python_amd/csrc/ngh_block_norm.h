@@ -78,6 +78,23 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a) {
             if (a.b) load_piece<T, VEC, RAGGED>((const T*)a.b + (long long)n * a.b_stride + col, in[c], inside, v[c]);
         }
     }
+    // Gains, biases and gate are asked for with the rows rather than behind the reductions, where each costs its
+    // latency again: 16384 rows of 4096 bf16 elements 98 us, 103 then.
+    float p[C][VEC], q[C][VEC], g[C][VEC], w[C][VEC], z[C][VEC];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const unsigned col = (c * lanes + lane) * VEC;
+        if (!in[c]) continue;
+        if (a.post) {
+            load_param<T, VEC, RAGGED>(a.post_gain, col, in[c], a.param_f32, 1.0f, p[c]);
+            load_param<T, VEC, RAGGED>(a.post_bias, col, in[c], a.param_f32, 0.0f, q[c]);
+        }
+        load_param<T, VEC, RAGGED>(a.gate, a.gate ? (long long)(n / a.gate_rows) * a.gate_stride + col : 0, in[c], a.param_f32, 1.0f, g[c]);
+        if (a.y) {
+            load_param<T, VEC, RAGGED>(a.gain, col, in[c], a.param_f32, 1.0f, w[c]);
+            load_param<T, VEC, RAGGED>(a.bias, col, in[c], a.param_f32, 0.0f, z[c]);
+        }
+    }
     if (a.post) {
         float mean = 0.0f;
         if (LAYER) {
@@ -101,13 +118,9 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a) {
         const float r = 1.0f / sqrtf(s[0] * a.inv_width + a.eps);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const unsigned col = (c * lanes + lane) * VEC;
-            float p[VEC], q[VEC];
             if (in[c]) {
-                load_param<T, VEC, RAGGED>(a.post_gain, col, in[c], a.param_f32, 1.0f, p);
-                load_param<T, VEC, RAGGED>(a.post_bias, col, in[c], a.param_f32, 0.0f, q);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) v[c][i] = v[c][i] * r * p[i] + q[i];
+                for (int i = 0; i < VEC; ++i) v[c][i] = v[c][i] * r * p[c][i] + q[c][i];
             }
         }
     }
@@ -115,10 +128,8 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a) {
     for (int c = 0; c < C; ++c) {
         const unsigned col = (c * lanes + lane) * VEC;
         if (in[c]) {
-            float g[VEC];
-            load_param<T, VEC, RAGGED>(a.gate, a.gate ? (long long)(n / a.gate_rows) * a.gate_stride + col : 0, in[c], a.param_f32, 1.0f, g);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) v[c][i] = a.alpha * x[c][i] + v[c][i] * g[i];
+            for (int i = 0; i < VEC; ++i) v[c][i] = a.alpha * x[c][i] + v[c][i] * g[c][i];
             if (a.h) store_piece<T, VEC, RAGGED>((T*)a.h + (long long)n * a.h_stride + col, in[c], v[c]);
         }
     }
@@ -147,11 +158,8 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a) {
     for (int c = 0; c < C; ++c) {
         const unsigned col = (c * lanes + lane) * VEC;
         if (in[c]) {
-            float w[VEC], z[VEC];
-            load_param<T, VEC, RAGGED>(a.gain, col, in[c], a.param_f32, 1.0f, w);
-            load_param<T, VEC, RAGGED>(a.bias, col, in[c], a.param_f32, 0.0f, z);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) v[c][i] = v[c][i] * r * w[i] + z[i];
+            for (int i = 0; i < VEC; ++i) v[c][i] = v[c][i] * r * w[c][i] + z[c][i];
             store_piece<T, VEC, RAGGED>((T*)a.y + (long long)n * a.y_stride + col, in[c], v[c]);
         }
     }

@@ -22,8 +22,14 @@ struct View {
 
 constexpr int kMostViews = 20;
 
-// Everything the call touches; returns how many.
-int views_of(const ngh_block_norm_spec* s, bool grad, View (&v)[kMostViews]) {
+struct Views {
+    View v[kMostViews];
+    int n = 0;
+};
+
+// Everything the call touches.
+void views_of(const ngh_block_norm_spec* s, bool grad, Views& views) {
+    View* v = views.v;
     const int e = size_of(s->dtype), q = size_of(s->param_dtype);
     const int64_t gates = s->gate_rows > 0 ? s->rows / s->gate_rows : 0;
     int n = 0;
@@ -52,10 +58,10 @@ int views_of(const ngh_block_norm_spec* s, bool grad, View (&v)[kMostViews]) {
         add("dgate", s->dgate, gates, s->dgate_stride, q, true);
         add("workspace", s->workspace, 1, (int64_t)s->workspace_bytes, 1, true);
     }
-    return n;
+    views.n = n;
 }
 
-int check(const ngh_block_norm_spec* s, bool grad, const char* what) {
+int check(const ngh_block_norm_spec* s, bool grad, const char* what, Views& views) {
     if (!s) return report(NGH_E_INVALID, "%s: spec is NULL", what);
     if (s->abi_version != NGH_ABI_VERSION)
         return report(NGH_E_INVALID, "%s: abi_version %d, this library is %d", what, s->abi_version, NGH_ABI_VERSION);
@@ -91,8 +97,9 @@ int check(const ngh_block_norm_spec* s, bool grad, const char* what) {
         if (!s->post_norm && (s->dpost_gain || s->dpost_bias)) return report(NGH_E_INVALID, "%s: a gradient of the norm after the block without post_norm", what);
         if (s->dgate && !s->gate) return report(NGH_E_INVALID, "%s: dgate without a gate", what);
     }
-    View v[kMostViews];
-    const int n = views_of(s, grad, v);
+    views_of(s, grad, views);
+    const View* v = views.v;
+    const int n = views.n;
     for (int i = 0; i < n; ++i) {
         if ((uintptr_t)v[i].p % v[i].item) return report(NGH_E_INVALID, "%s: %s is not aligned to its elements", what, v[i].name);
         if (v[i].rows > 1 && v[i].stride < s->width) return report(NGH_E_INVALID, "%s: stride %lld of %s below the width", what, (long long)v[i].stride, v[i].name);
@@ -113,10 +120,10 @@ int check(const ngh_block_norm_spec* s, bool grad, const char* what) {
     return NGH_OK;
 }
 
-NormShape shape_of(const ngh_block_norm_spec* s, bool grad) {
+NormShape shape_of(const ngh_block_norm_spec* s, const Views& views) {
     NormShape f;
-    View v[kMostViews];
-    const int n = views_of(s, grad, v);
+    const View* v = views.v;
+    const int n = views.n;
     const int vec = 16 / size_of(s->dtype);
     bool whole = s->width % vec == 0;
     for (int i = 0; i < n; ++i) {
@@ -168,18 +175,18 @@ struct GradPlan {
     size_t part_stride, bytes;
 };
 
-GradPlan plan_grad(const ngh_block_norm_spec* s, int cus) {
+GradPlan plan_grad(const ngh_block_norm_spec* s, const Views& views, int cus) {
     GradPlan g;
-    g.shape = shape_of(s, true);
+    g.shape = shape_of(s, views);
     g.vectors = (s->dgain ? kVecGain : 0) | (s->dbias ? kVecBias : 0) | (s->dpost_gain ? kVecPostGain : 0) | (s->dpost_bias ? kVecPostBias : 0);
     g.bias = s->dbias || s->dpost_bias;
     const unsigned rows = (unsigned)s->rows;
     // 16 wavefronts a compute unit (what the registers allow; a workgroup of 5 takes the room of 8), but at least
-    // 8 rows a part, for a part's sums are written in fp32 and read once more; fewer, down to 2, where else
+    // 8 rows a part, for a part's sums are written in fp32 and read once more; fewer, down to 1, where else
     // compute units would have no part.
     const unsigned groups = g.shape.rows_a_workgroup();
     const unsigned want = 1024u / ((g.shape.threads() + 255u) / 256u * 256u) * cus;
-    const unsigned least = std::min(8u, std::max(2u, rows / (2u * cus)));
+    const unsigned least = std::min(8u, std::max(1u, rows / (2u * cus)));
     g.per_part = std::max(least, (rows + want - 1) / want);
     g.per_group = (g.per_part + groups - 1) / groups;
     const unsigned gate_rows = (unsigned)std::max<int64_t>(1, s->gate_rows);
@@ -221,16 +228,18 @@ using namespace ngh;
 extern "C" {
 
 int ngh_validate_block_norm(const ngh_block_norm_spec* spec, int32_t gradient) {
-    return check(spec, gradient != 0, gradient ? "ngh_block_norm_grad" : "ngh_block_norm");
+    Views views;
+    return check(spec, gradient != 0, gradient ? "ngh_block_norm_grad" : "ngh_block_norm", views);
 }
 
 int ngh_block_norm(ngh_context* ctx, const ngh_block_norm_spec* spec) {
-    const int rc = ctx ? check(spec, false, "ngh_block_norm") : report(NGH_E_INVALID, "ctx is NULL");
+    Views views;
+    const int rc = ctx ? check(spec, false, "ngh_block_norm", views) : report(NGH_E_INVALID, "ctx is NULL");
     if (rc != NGH_OK || spec->rows == 0) return rc;
     const ContextView c = view_of(ctx);
     DeviceScope scope(c.device);
     if (!scope.ok()) return report(NGH_E_RUNTIME, "ngh_block_norm: the context's device cannot be made current");
-    const NormShape f = shape_of(spec, false);
+    const NormShape f = shape_of(spec, views);
     NormArgs a;
     fill_args(spec, f, a);
     const unsigned per_wg = f.rows_a_workgroup();
@@ -240,22 +249,24 @@ int ngh_block_norm(ngh_context* ctx, const ngh_block_norm_spec* spec) {
 int ngh_block_norm_grad_workspace(const ngh_block_norm_spec* spec, size_t* out_bytes) {
     if (!out_bytes) return report(NGH_E_INVALID, "ngh_block_norm_grad_workspace: out_bytes is NULL");
     *out_bytes = 0;
-    const int rc = check(spec, true, "ngh_block_norm_grad_workspace");
+    Views views;
+    const int rc = check(spec, true, "ngh_block_norm_grad_workspace", views);
     if (rc != NGH_OK) return rc;
     // (how the rows are dealt depends on the device's compute units; enough for any number of them)
     size_t most = 256;
-    for (int cus = 1; spec->rows && cus <= 1024; cus *= 2) most = std::max(most, plan_grad(spec, cus).bytes);
+    for (int cus = 1; spec->rows && cus <= 1024; cus *= 2) most = std::max(most, plan_grad(spec, views, cus).bytes);
     *out_bytes = most;
     return NGH_OK;
 }
 
 int ngh_block_norm_grad(ngh_context* ctx, const ngh_block_norm_spec* spec) {
-    const int rc = ctx ? check(spec, true, "ngh_block_norm_grad") : report(NGH_E_INVALID, "ctx is NULL");
+    Views views;
+    const int rc = ctx ? check(spec, true, "ngh_block_norm_grad", views) : report(NGH_E_INVALID, "ctx is NULL");
     if (rc != NGH_OK) return rc;
     const ContextView c = view_of(ctx);
     DeviceScope scope(c.device);
     if (!scope.ok()) return report(NGH_E_RUNTIME, "ngh_block_norm_grad: the context's device cannot be made current");
-    const GradPlan g = plan_grad(spec, c.cus);
+    const GradPlan g = plan_grad(spec, views, c.cus);
     if (spec->workspace_bytes < g.bytes || (g.bytes && !spec->workspace))
         return report(NGH_E_INVALID, "ngh_block_norm_grad: workspace of %zu bytes, %zu needed", spec->workspace_bytes, g.bytes);
     if ((uintptr_t)spec->workspace % 16) return report(NGH_E_INVALID, "ngh_block_norm_grad: misaligned workspace");

@@ -16,7 +16,8 @@
 //      summed by a wavefront for each block of columns, row after row in fp32.  A token all of whose
 //      rows lie in one unit is finished there; parts of a token that crosses units go to the
 //      workspace, so that one frequent token is spread over as many wavefronts as many rare ones.
-//      In the same launch other workgroups clear the rows whose token the sorted list does not hold.
+//      In the same launch other workgroups clear the rows whose token the sorted list does not hold; the
+//      launches of the sort, which leave the memory idle, have cleared the table's first rows altogether.
 //   3. merge.  A workgroup for each unit in which a crossing token begins adds its parts in order.
 #include <hip/hip_runtime.h>
 
@@ -33,6 +34,7 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / 64;
 constexpr int kRankMax = 16384;                          // places sorted by chunks: 64 KiB of keys in LDS
 constexpr int kChunk = 2048;
+constexpr int kOneChunk = 4096;                          // up to here one chunk holds all places
 constexpr int kFew = 2048;                               // places that need no sort
 constexpr int kFewWaves = 8;
 constexpr int kFewAlone = 16;                            // rows a wavefront adds by itself (one batch in flight)
@@ -110,7 +112,22 @@ struct SortArgs {
     unsigned* table;             // [tiles][kTileDigits] counts of this pass
     unsigned tiles;
     int shift, bits;
+    // workgroups behind the first `workers` clear [clear, clear + clear_bytes), from a 16-byte boundary
+    unsigned workers;
+    char* clear;
+    unsigned long long clear_bytes;
 };
+
+// Workgroups of a launch of the sort that do not sort: each clears its share of a part of the table.
+__device__ __forceinline__ bool clears(const SortArgs& a) {
+    if (blockIdx.x < a.workers) return false;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    uint4* p = reinterpret_cast<uint4*>(a.clear);
+    for (unsigned long long i = (unsigned long long)(blockIdx.x - a.workers) * blockDim.x + threadIdx.x; i < a.clear_bytes / 16;
+         i += (unsigned long long)(gridDim.x - a.workers) * blockDim.x)
+        p[i] = zero;
+    return true;
+}
 
 // A token that takes part in no sum sorts behind all others.
 __device__ __forceinline__ unsigned key_of(int t, unsigned vocab, int pad) {
@@ -145,19 +162,21 @@ __device__ __forceinline__ unsigned scan_exclusive(unsigned v, unsigned* sh) {
     return before + s - v;
 }
 
-// All pairs within chunks of kChunk places: a workgroup ranks 64 places, one a lane; its wavefronts share
+// All pairs within chunks of CHUNK places: a workgroup ranks 64 places, one a lane; its wavefronts share
 // the places of the chunk they are compared with, which lie in LDS as keys.  Equal keys rank in order of
-// their places.  Two to three instructions a pair: 2 us for a chunk, whatever the number of chunks.
+// their places.  Two to three instructions a pair: 2.5 us for chunks of 2048, whatever their number.
+template <int CHUNK>
 __global__ __launch_bounds__(kSortThreads) void rank_chunk_kernel(SortArgs a) {
-    __shared__ uint4 keys4[kChunk / 4];
+    __shared__ uint4 keys4[CHUNK / 4];
+    if (clears(a)) return;
     unsigned* keys = reinterpret_cast<unsigned*>(keys4);
-    const unsigned first = blockIdx.x * 64 / kChunk * kChunk;        // of the chunk
-    for (unsigned i = threadIdx.x; i < kChunk; i += kSortThreads)
+    const unsigned first = blockIdx.x * 64 / CHUNK * CHUNK;        // of the chunk
+    for (unsigned i = threadIdx.x; i < CHUNK; i += kSortThreads)
         keys[i] = first + i < a.n ? key_of(a.tokens[first + i], a.vocab, a.pad) : ~0u;
     __syncthreads();
     const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned base = blockIdx.x * 64 - first, mine = keys[base + lane];
-    constexpr unsigned kEach = kChunk / kSortWaves;
+    constexpr unsigned kEach = CHUNK / kSortWaves;
     unsigned count = 0;
     for (unsigned c = wave * kEach; c < (wave + 1) * kEach; c += 64) {
         const uint4* k4 = keys4 + c / 4;
@@ -197,6 +216,7 @@ __global__ __launch_bounds__(kSortThreads) void rank_chunk_kernel(SortArgs a) {
 // it (chunks behind) or not above it (chunks in front), found by halving in all chunks at once.
 __global__ __launch_bounds__(kEmbBlock) void rank_join_kernel(SortArgs a) {
     __shared__ unsigned keys[kRankMax];
+    if (clears(a)) return;
     constexpr int kChunks = kRankMax / kChunk;
     const unsigned i = blockIdx.x * kEmbBlock + threadIdx.x;
     const unsigned place = i < a.n ? a.place_in[i] : 0u;
@@ -241,6 +261,7 @@ __device__ __forceinline__ unsigned tile_key(const SortArgs& a, unsigned i) {
 template <bool FIRST>
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a) {
     __shared__ unsigned hist[kTileDigits];
+    if (clears(a)) return;
     for (unsigned i = threadIdx.x; i < kTileDigits; i += kSortThreads) hist[i] = 0;
     __syncthreads();
 #pragma unroll
@@ -260,6 +281,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortArgs a) 
     __shared__ unsigned start[kTileDigits];
     __shared__ unsigned part[kTileDigits];
     __shared__ unsigned sh[kSortWaves];
+    if (clears(a)) return;
     const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const unsigned digits = 1u << a.bits;
     unsigned key[kTileItems], place[kTileItems], rank[kTileItems];
@@ -340,6 +362,7 @@ struct SumArgs {
     long long dy_stride, table_stride, part_stride;
     unsigned n, vocab, width, units, unit;
     unsigned workers, slab;    // workgroups that add; behind them one for every `slab` rows of the table to clear
+    unsigned cleared;          // rows of the table that are clear already
     float scale;
     int accumulate;
 };
@@ -401,7 +424,7 @@ __global__ __launch_bounds__(kEmbBlock) void embedding_sum_kernel(SumArgs a, uns
     typedef typename VecOf<TIn, VEC>::type Raw;
     typedef typename VecOf<TOut, VEC>::type Old;
     if (!ADD && blockIdx.x >= a.workers) {
-        const unsigned r0 = ((blockIdx.x - a.workers) * (kEmbBlock / 64) + (threadIdx.x >> 6)) * a.slab;
+        const unsigned r0 = a.cleared + ((blockIdx.x - a.workers) * (kEmbBlock / 64) + (threadIdx.x >> 6)) * a.slab;
         if (r0 < a.vocab) clear_missing<TOut, RAGGED>(a, r0, min(a.slab, a.vocab - r0));
         return;
     }
@@ -777,10 +800,11 @@ GradPlan plan_grad(const ngh_embedding_spec* s, int cus) {
 
 // Workgroups that clear the table, a.slab rows for each of `parts` parts of one: about `wgs` of them.
 unsigned slabs_of(SumArgs& a, unsigned wgs, unsigned most, unsigned parts) {
-    if (a.accumulate || a.vocab == 0) return 0;
-    a.slab = std::min(most, std::max(1u, (a.vocab + wgs * parts - 1) / (wgs * parts)));
+    const unsigned rows = a.vocab - a.cleared;
+    if (a.accumulate || rows == 0) return 0;
+    a.slab = std::min(most, std::max(1u, (rows + wgs * parts - 1) / (wgs * parts)));
     const unsigned per = a.slab * parts;
-    return (a.vocab + per - 1) / per;
+    return (rows + per - 1) / per;
 }
 
 template <class TIn, class TOut, bool RAGGED>
@@ -889,17 +913,38 @@ int ngh_embedding_grad(ngh_context* ctx, const ngh_embedding_spec* spec) {
     s.pad = spec->pad_idx;
     s.tiles = g.tiles;
     s.table = (unsigned*)(ws + g.tables);
+    // What a launch that ranks chunks clears beside it: 64 MiB at most, in whole rows, eight at a time so that the next
+    // part starts on 16 bytes too ([65536, 1024] fp32: 82 -> 79 us with 16384 places, 69 -> 57 with 2100; beside the
+    // longer sort by tiles it gained nothing).
+    const unsigned long long row_bytes = (unsigned long long)spec->width * te;
+    const bool dense = (spec->table_stride == spec->width || spec->vocab == 1) && (uintptr_t)spec->table % 16 == 0;
+    const unsigned part_rows = spec->accumulate || !dense || g.tiles ? 0u : (unsigned)std::min<unsigned long long>((64ull << 20) / row_bytes / 8 * 8, spec->vocab);
+    unsigned cleared = 0;
+    auto launch_sort = [&](auto kernel, unsigned workers, unsigned threads) {
+        const unsigned rows = std::min(part_rows, (s.vocab - cleared) / 8 * 8);
+        s.workers = workers;
+        s.clear = (char*)spec->table + cleared * row_bytes;
+        s.clear_bytes = rows * row_bytes;
+        cleared += rows;
+        const unsigned extra = (unsigned)std::min<unsigned long long>((s.clear_bytes + 16 * threads - 1) / (16 * threads), 2u * c.cus);
+        hipLaunchKernelGGL(kernel, dim3(workers + extra), dim3(threads), 0, c.stream, s);
+        return hipGetLastError();
+    };
     if (!g.few && g.tiles == 0) {
-        s.key_out = (unsigned*)(ws + g.keys_b);
-        s.place_out = (unsigned*)(ws + g.places_b);
-        hipLaunchKernelGGL(rank_chunk_kernel, dim3((s.n + 63) / 64), dim3(kSortThreads), 0, c.stream, s);
-        NGH_HIP_TRY(hipGetLastError());
-        s.key_in = s.key_out;
-        s.place_in = s.place_out;
-        s.key_out = (unsigned*)(ws + g.keys_a);
-        s.place_out = (unsigned*)(ws + g.places_a);
-        hipLaunchKernelGGL(rank_join_kernel, dim3((s.n + kEmbBlock - 1) / kEmbBlock), dim3(kEmbBlock), 0, c.stream, s);
-        NGH_HIP_TRY(hipGetLastError());
+        // one launch while that is cheaper than a second one (4096 places: 8 us, 14 in two)
+        const bool one = s.n <= (unsigned)kOneChunk;
+        s.key_out = (unsigned*)(ws + (one ? g.keys_a : g.keys_b));
+        s.place_out = (unsigned*)(ws + (one ? g.places_a : g.places_b));
+        const unsigned workers = (s.n + 63) / 64;
+        if (one) NGH_HIP_TRY(launch_sort(rank_chunk_kernel<kOneChunk>, workers, kSortThreads));
+        else NGH_HIP_TRY(launch_sort(rank_chunk_kernel<kChunk>, workers, kSortThreads));
+        if (!one) {
+            s.key_in = s.key_out;
+            s.place_in = s.place_out;
+            s.key_out = (unsigned*)(ws + g.keys_a);
+            s.place_out = (unsigned*)(ws + g.places_a);
+            NGH_HIP_TRY(launch_sort(rank_join_kernel, (s.n + kEmbBlock - 1) / kEmbBlock, kEmbBlock));
+        }
     } else if (!g.few) {
         const int digit = (g.bits + g.passes - 1) / g.passes;
         for (int p = 0; p < g.passes; ++p) {
@@ -911,13 +956,12 @@ int ngh_embedding_grad(ngh_context* ctx, const ngh_embedding_spec* spec) {
             s.key_in = (const unsigned*)(ws + (a_out ? g.keys_b : g.keys_a));
             s.place_in = (const unsigned*)(ws + (a_out ? g.places_b : g.places_a));
             if (p == 0) {
-                hipLaunchKernelGGL(sort_count_kernel<true>, dim3(g.tiles), dim3(kSortThreads), 0, c.stream, s);
-                hipLaunchKernelGGL(sort_scatter_kernel<true>, dim3(g.tiles), dim3(kSortThreads), 0, c.stream, s);
+                NGH_HIP_TRY(launch_sort(sort_count_kernel<true>, g.tiles, kSortThreads));
+                NGH_HIP_TRY(launch_sort(sort_scatter_kernel<true>, g.tiles, kSortThreads));
             } else {
-                hipLaunchKernelGGL(sort_count_kernel<false>, dim3(g.tiles), dim3(kSortThreads), 0, c.stream, s);
-                hipLaunchKernelGGL(sort_scatter_kernel<false>, dim3(g.tiles), dim3(kSortThreads), 0, c.stream, s);
+                NGH_HIP_TRY(launch_sort(sort_count_kernel<false>, g.tiles, kSortThreads));
+                NGH_HIP_TRY(launch_sort(sort_scatter_kernel<false>, g.tiles, kSortThreads));
             }
-            NGH_HIP_TRY(hipGetLastError());
         }
     }
     SumArgs a{};
@@ -932,6 +976,7 @@ int ngh_embedding_grad(ngh_context* ctx, const ngh_embedding_spec* spec) {
     a.n = (unsigned)spec->rows;
     a.vocab = (unsigned)spec->vocab;
     a.width = (unsigned)spec->width;
+    a.cleared = cleared;
     a.units = g.units;
     a.unit = g.unit;
     a.scale = spec->scale;

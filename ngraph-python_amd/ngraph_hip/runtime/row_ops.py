@@ -144,10 +144,14 @@ class OperatorCalls(object):
         return s
 
     def embedding(self, spec):
-        self._check(self.lib.ngh_embedding(self.ctx, ctypes.byref(spec)))
+        rc = self.lib.ngh_embedding(self.ctx, spec)
+        if rc:
+            self._check(rc)
 
     def embedding_grad(self, spec):
-        self._check(self.lib.ngh_embedding_grad(self.ctx, ctypes.byref(spec)))
+        rc = self.lib.ngh_embedding_grad(self.ctx, spec)
+        if rc:
+            self._check(rc)
 
     def embedding_grad_workspace(self, spec):
         """Bytes of device memory embedding_grad(spec) works in."""
@@ -181,10 +185,14 @@ class OperatorCalls(object):
         return s
 
     def block_norm(self, spec):
-        self._check(self.lib.ngh_block_norm(self.ctx, ctypes.byref(spec)))
+        rc = self.lib.ngh_block_norm(self.ctx, spec)
+        if rc:
+            self._check(rc)
 
     def block_norm_grad(self, spec):
-        self._check(self.lib.ngh_block_norm_grad(self.ctx, ctypes.byref(spec)))
+        rc = self.lib.ngh_block_norm_grad(self.ctx, spec)
+        if rc:
+            self._check(rc)
 
     def block_norm_grad_workspace(self, spec):
         """Bytes of device memory block_norm_grad(spec) works in."""
