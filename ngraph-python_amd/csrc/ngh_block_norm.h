@@ -65,18 +65,14 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a) {
     const bool live = row < a.rows;                      // (idle lanes still take part in the reductions)
     const unsigned n = live ? row : 0;
     const bool inside = n + 1 < a.rows && a.width >= VEC;
-    float v[C][VEC], x[C][VEC];
+    typename VecOf<T, VEC>::type rx[C], rb[C];
     int in[C];                                           // elements of each piece
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const unsigned col = (c * lanes + lane) * VEC;
         in[c] = live ? piece_count<VEC, RAGGED>(col, a.width) : 0;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[c][i] = x[c][i] = 0.0f;
-        if (in[c]) {
-            load_piece<T, VEC, RAGGED>((const T*)a.x + (long long)n * a.x_stride + col, in[c], inside, x[c]);
-            if (a.b) load_piece<T, VEC, RAGGED>((const T*)a.b + (long long)n * a.b_stride + col, in[c], inside, v[c]);
-        }
+        rx[c] = load_raw<T, VEC, RAGGED>((const T*)a.x + (long long)n * a.x_stride + col, in[c], inside);
+        rb[c] = load_raw<T, VEC, RAGGED>((const T*)a.b + (long long)n * a.b_stride + col, a.b ? in[c] : 0, inside);
     }
     // Gains, biases and gate are asked for with the rows rather than behind the reductions, where each costs its
     // latency again: 16384 rows of 4096 bf16 elements 98 us, 103 then.
@@ -94,6 +90,12 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a) {
             load_param<T, VEC, RAGGED>(a.gain, col, in[c], a.param_f32, 1.0f, w[c]);
             load_param<T, VEC, RAGGED>(a.bias, col, in[c], a.param_f32, 0.0f, z[c]);
         }
+    }
+    float v[C][VEC], x[C][VEC];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        to_float<T, VEC, RAGGED>(rx[c], in[c], x[c]);
+        to_float<T, VEC, RAGGED>(rb[c], in[c], v[c]);
     }
     if (a.post) {
         float mean = 0.0f;
@@ -246,14 +248,12 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4))) vo
         const unsigned n = first + turn;
         float h[C][VEC], t[C][VEC], b[C][VEC], d[C][VEC];
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                h[c][i] = (float)rh[c][i];
-                t[c][i] = (float)rt[c][i];
-                b[c][i] = (float)rb[c][i];
-                d[c][i] = (float)rd[c][i];
-            }
+        for (int c = 0; c < C; ++c) {
+            to_float<T, VEC, RAGGED>(rh[c], in[c], h[c]);
+            to_float<T, VEC, RAGGED>(rt[c], in[c], t[c]);
+            to_float<T, VEC, RAGGED>(rb[c], in[c], b[c]);
+            to_float<T, VEC, RAGGED>(rd[c], in[c], d[c]);
+        }
         fetch(n + 1, n + 1 < last);
         float brs = 1.0f;
         if (LAYER) {
@@ -486,10 +486,10 @@ __global__ __launch_bounds__(1024) void block_norm_merge_kernel(NormMergeArgs a)
     else ((T*)a.out[vec])[col] = (T)acc;
 }
 
-// The shape of the kernel that a row takes: C pieces of VEC elements a lane on `lanes` lanes (whole wavefronts,
-// or a power of two up to 64).  ragged: rows that do not start, or end, on 16-byte boundaries.
+// The shape of the kernel that a row takes: `pieces` pieces of `vec` elements a lane on `lanes` lanes (whole
+// wavefronts, or a power of two up to 64).  ragged: rows that do not start, or end, on 16-byte boundaries.
 struct NormShape {
-    int pieces, lanes;
+    int vec, pieces, lanes;
     bool ragged;
     bool several() const { return lanes > 64; }
     unsigned threads() const { return several() ? (unsigned)lanes : 256u; }
@@ -513,10 +513,24 @@ void launch_norm_kernel(const NormShape& s, const NormArgs& a, NormPass pass, un
 }
 
 // The pieces a lane may hold: one (rows of up to 16 KiB: at most 1024 lanes), two, and four of 4 elements.
+// Pieces of 4 elements where 16 bytes are 8: only what shape_of asks for (ragged rows, backward).
 template <class T, bool RAGGED, bool LAYER>
 int launch_norm_shape(const NormShape& s, const NormArgs& a, NormPass pass, unsigned grid, hipStream_t stream) {
     constexpr int kVec = 16 / sizeof(T);
-    if (s.pieces == 1) {
+    if (s.vec != kVec) {
+        if constexpr (RAGGED && kVec == 8) {
+            const dim3 block(s.threads());
+            const unsigned lds = (unsigned)__builtin_popcount((unsigned)a.in_lds) * a.lds_stride * 4;
+            if (!s.several() && pass == kNormBackward)
+                hipLaunchKernelGGL((block_norm_grad_kernel<T, 4, 1, 256, false, true, LAYER, false>), dim3(grid), block, lds, stream, a);
+            else if (!s.several())
+                hipLaunchKernelGGL((block_norm_grad_kernel<T, 4, 1, 256, false, true, LAYER, true>), dim3(grid), block, lds, stream, a);
+            else if (s.lanes <= 512)
+                hipLaunchKernelGGL((block_norm_grad_kernel<T, 4, 1, 512, true, true, LAYER, true>), dim3(grid), block, lds, stream, a);
+            else
+                hipLaunchKernelGGL((block_norm_grad_kernel<T, 4, 1, 1024, true, true, LAYER, true>), dim3(grid), block, lds, stream, a);
+        }
+    } else if (s.pieces == 1) {
         if (!s.several()) launch_norm_kernel<T, kVec, 1, 256, false, RAGGED, LAYER>(s, a, pass, grid, stream);
         else if (s.lanes <= 256) launch_norm_kernel<T, kVec, 1, 256, true, RAGGED, LAYER>(s, a, pass, grid, stream);
         else if (s.lanes <= 512) launch_norm_kernel<T, kVec, 1, 512, true, RAGGED, LAYER>(s, a, pass, grid, stream);

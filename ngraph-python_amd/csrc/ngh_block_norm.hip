@@ -120,7 +120,7 @@ int check(const ngh_block_norm_spec* s, bool grad, const char* what, Views& view
     return NGH_OK;
 }
 
-NormShape shape_of(const ngh_block_norm_spec* s, const Views& views) {
+NormShape shape_of(const ngh_block_norm_spec* s, const Views& views, NormPass pass) {
     NormShape f;
     const View* v = views.v;
     const int n = views.n;
@@ -132,9 +132,13 @@ NormShape shape_of(const ngh_block_norm_spec* s, const Views& views) {
         whole = whole && (uintptr_t)v[i].p % piece == 0 && (v[i].rows <= 1 || v[i].stride * v[i].item % piece == 0);
     }
     f.ragged = !whole;
+    // Backward, ragged rows of 16 bits: pieces of 8 elements do not fit the registers with the sums of the biases
+    // (16384 layer norms of 2050 bf16 elements 302 us, 234 with pieces of 4; without those sums 158 and 235), nor
+    // where rows share a wavefront (65536 rows of 100: 52 and 34 us; of 250: 71 and 63).
+    f.vec = f.ragged && ((pass == kNormBackward && s->width <= 64 * 4) || (pass == kNormBackwardBias && s->width <= 1024 * 4)) ? 4 : vec;
     f.pieces = 1;
-    while (1024 * vec * f.pieces < s->width) f.pieces *= 2;
-    const int per_lane = vec * f.pieces;
+    while (1024 * f.vec * f.pieces < s->width) f.pieces *= 2;
+    const int per_lane = f.vec * f.pieces;
     f.lanes = 1;
     while (f.lanes < 64 && f.lanes * per_lane < s->width) f.lanes *= 2;
     if (f.lanes * per_lane < s->width) f.lanes = (int)((s->width + per_lane * 64 - 1) / (per_lane * 64)) * 64;
@@ -177,9 +181,9 @@ struct GradPlan {
 
 GradPlan plan_grad(const ngh_block_norm_spec* s, const Views& views, int cus) {
     GradPlan g;
-    g.shape = shape_of(s, views);
     g.vectors = (s->dgain ? kVecGain : 0) | (s->dbias ? kVecBias : 0) | (s->dpost_gain ? kVecPostGain : 0) | (s->dpost_bias ? kVecPostBias : 0);
     g.bias = s->dbias || s->dpost_bias;
+    g.shape = shape_of(s, views, g.bias ? kNormBackwardBias : kNormBackward);
     const unsigned rows = (unsigned)s->rows;
     // 16 wavefronts a compute unit (what the registers allow; a workgroup of 5 takes the room of 8), but at least
     // 8 rows a part, for a part's sums are written in fp32 and read once more; fewer, down to 1, where else
@@ -239,7 +243,7 @@ int ngh_block_norm(ngh_context* ctx, const ngh_block_norm_spec* spec) {
     const ContextView c = view_of(ctx);
     DeviceScope scope(c.device);
     if (!scope.ok()) return report(NGH_E_RUNTIME, "ngh_block_norm: the context's device cannot be made current");
-    const NormShape f = shape_of(spec, views);
+    const NormShape f = shape_of(spec, views, kNormForward);
     NormArgs a;
     fill_args(spec, f, a);
     const unsigned per_wg = f.rows_a_workgroup();

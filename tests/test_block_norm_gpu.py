@@ -353,3 +353,35 @@ def test_recorded_calls_replay_with_new_rows(hip_runtime):
                     np.testing.assert_array_equal(replayed[n], tensors[n].get(), err_msg=n)
         finally:
             rt.graph_free(graph)
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("types", [("f16", "f16"), ("bf16", "f32"), ("bf16", "bf16")], ids="-".join)
+@pytest.mark.parametrize("rows,width", [(40, 250), (9, 257), (22, 2049), (7, 2051), (3, 4095), (3, 4097)])
+def test_odd_rows_with_all_sums(hip_runtime, rows, width, types, kind):
+    """Rows of 16 bits on any boundary with the gradients of biases: the widths where the pieces a lane holds change."""
+    run_backward(hip_runtime, Case(rows, width, kind, types, gate_rows=rows, bias=True, seed=rows), runs=2)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("width", [35, 130, 515, 2051])
+def test_not_a_number_stays_in_its_row_backward(hip_runtime, dtype, width):
+    """What a short last piece reads of the next row is no part of its own."""
+    rt, rs = hip_runtime, np.random.RandomState(width)
+    clean = {n: rounded(rs.normal(0, 1, (5, width)), dtype) for n in ("h", "b", "dy", "dh")}
+    kept = {}
+    for bad in (False, True):
+        values = {n: v.copy() for n, v in clean.items()}
+        if bad:
+            for v in values.values():
+                v[1], v[3] = np.nan, np.inf
+        with Pool(rt) as pool:
+            tensors = {n: pool.rows((5, width), dtype, v) for n, v in values.items()}
+            tensors.update({n: pool.rows((5, width), dtype) for n in ("dx", "db")})
+            names = {n: t.ptr for n, t in tensors.items()}
+            names.update({n + "_stride": width for n in tensors})
+            rt.block_norm_grad(rt.block_norm_spec(5, width, "layer", DTYPES[dtype], DTYPES[dtype], True, **names))
+            kept[bad] = {n: tensors[n].get() for n in ("dx", "db")}
+    for n in ("dx", "db"):
+        assert np.isnan(kept[True][n][[1, 3]]).all(), n
+        np.testing.assert_array_equal(kept[True][n][[0, 2, 4]], kept[False][n][[0, 2, 4]], err_msg=n)
