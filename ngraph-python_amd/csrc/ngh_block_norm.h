@@ -27,6 +27,7 @@ struct NormArgs {
     float* parts;                  // backward: [part][vector][part_stride] sums of a part's rows
     long long x_stride, b_stride, gate_stride, h_stride, y_stride, dy_stride, dh_stride, dx_stride, db_stride, dgate_stride, part_stride;
     unsigned rows, width, gate_rows;
+    unsigned first_row;            // forward: of this launch
     int lanes;                     // along a row: whole wavefronts, or a power of two up to 64
     int post, param_f32;
     float eps, alpha, inv_width, width_f;      // (a mean is a quotient: a row of equal elements is all zeros behind it)
@@ -61,7 +62,7 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a) {
     clear_row_sums<SEVERAL>(sh);
     const unsigned lanes = a.lanes;
     const unsigned lane = SEVERAL ? threadIdx.x : threadIdx.x & (lanes - 1);
-    const unsigned row = SEVERAL ? blockIdx.x : blockIdx.x * (THREADS / lanes) + threadIdx.x / lanes;
+    const unsigned row = a.first_row + (SEVERAL ? blockIdx.x : blockIdx.x * (THREADS / lanes) + threadIdx.x / lanes);
     const bool live = row < a.rows;                      // (idle lanes still take part in the reductions)
     const unsigned n = live ? row : 0;
     const bool inside = n + 1 < a.rows && a.width >= VEC;

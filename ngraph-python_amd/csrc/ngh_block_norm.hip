@@ -80,7 +80,7 @@ int check(const ngh_block_norm_spec* s, bool grad, const char* what, Views& view
     if (!s->post_norm && (s->post_gain || s->post_bias))
         return report(NGH_E_INVALID, "%s: a gain or bias after the block without post_norm", what);
     if (s->gate) {
-        if (s->gate_rows < 1 || s->rows % s->gate_rows) return report(NGH_E_INVALID, "%s: gate_rows %lld of %lld rows", what, (long long)s->gate_rows, (long long)s->rows);
+        if (s->gate_rows < 1 || s->gate_rows >= (1LL << 31) || s->rows % s->gate_rows) return report(NGH_E_INVALID, "%s: gate_rows %lld of %lld rows", what, (long long)s->gate_rows, (long long)s->rows);
     } else if (s->gate_rows) {
         return report(NGH_E_INVALID, "%s: gate_rows without a gate", what);
     }
@@ -247,7 +247,12 @@ int ngh_block_norm(ngh_context* ctx, const ngh_block_norm_spec* spec) {
     NormArgs a;
     fill_args(spec, f, a);
     const unsigned per_wg = f.rows_a_workgroup();
-    return launch(spec, f, a, kNormForward, (a.rows + per_wg - 1) / per_wg, c.stream);
+    const unsigned slice = (unsigned)(kMostThreads / f.threads()) * per_wg;
+    for (; a.first_row < a.rows; a.first_row += std::min(slice, a.rows - a.first_row)) {
+        const int lrc = launch(spec, f, a, kNormForward, (std::min(slice, a.rows - a.first_row) + per_wg - 1) / per_wg, c.stream);
+        if (lrc != NGH_OK) return lrc;
+    }
+    return NGH_OK;
 }
 
 int ngh_block_norm_grad_workspace(const ngh_block_norm_spec* spec, size_t* out_bytes) {

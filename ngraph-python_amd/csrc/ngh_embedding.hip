@@ -10,8 +10,8 @@
 // clear the rows of the table whose token does not occur.  More places are sorted by (token, place) first:
 //   1. sort.  Up to kRankMax places: chunks of kChunk are ranked by all pairs, then every place looks
 //      its rank up in the other chunks.  More: tiles of kTile places, sorted by the token's bits as
-//      digits, least significant first, each pass stable: a launch that counts a tile's digits and one
-//      that ranks and scatters.
+//      digits, least significant first, each pass stable: a launch that counts a tile's digits, where
+//      there are many tiles one that adds the counts up, and one that ranks and scatters.
 //   2. sums.  The sorted list is cut into units of equal length, whatever the tokens are: a unit is
 //      summed by a wavefront for each block of columns, row after row in fp32.  A token all of whose
 //      rows lie in one unit is finished there; parts of a token that crosses units go to the
@@ -43,6 +43,9 @@ constexpr int kTileItems = 2;
 constexpr int kTile = kSortThreads * kTileItems;
 constexpr int kTileDigitBits = 9;
 constexpr int kTileDigits = 1 << kTileDigitBits;
+// Up to here every tile adds the counts of those before it itself (of 64 elements a row: 131072 places 60 us,
+// 64 with a launch that does it for all; 1048576 places 204 and 177 us).
+constexpr int kTilesUnscanned = 128;
 
 // ---- lookup ----------------------------------------------------------------------------------
 struct LookupArgs {
@@ -109,8 +112,9 @@ struct SortArgs {
     const unsigned* place_in;
     unsigned* key_out;
     unsigned* place_out;
-    unsigned* table;             // [tiles][kTileDigits] counts of this pass
-    unsigned tiles;
+    unsigned* table;             // [tiles][kTileDigits] counts of this pass; with `scanned` those of the tiles
+                                 // before, and a row of all tiles'
+    unsigned tiles, scanned;
     int shift, bits;
     // workgroups behind the first `workers` clear [clear, clear + clear_bytes), from a 16-byte boundary
     unsigned workers;
@@ -273,6 +277,41 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a) {
     for (unsigned i = threadIdx.x; i < kTileDigits; i += kSortThreads) a.table[blockIdx.x * kTileDigits + i] = hist[i];
 }
 
+// Many tiles: a digit's counts become those of the tiles before, and row `tiles` holds those of all.  A
+// workgroup has 16 digits (a 64-byte piece of a row) and 64 lanes a digit, each with a run of tiles.
+constexpr int kScanDigits = 16;
+
+__global__ __launch_bounds__(kSortThreads) void sort_scan_kernel(SortArgs a) {
+    constexpr unsigned kRuns = kSortThreads / kScanDigits;
+    __shared__ unsigned sums[kRuns][kScanDigits + 1];
+    const unsigned x = threadIdx.x % kScanDigits, y = threadIdx.x / kScanDigits;
+    const unsigned each = (a.tiles + kRuns - 1) / kRuns, first = min(a.tiles, y * each), last = min(a.tiles, first + each);
+    unsigned* column = a.table + blockIdx.x * kScanDigits + x;
+    unsigned sum = 0;
+    for (unsigned t = first; t < last; t += 8) {
+        unsigned c[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) c[k] = t + k < last ? column[(size_t)(t + k) * kTileDigits] : 0u;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum += c[k];
+    }
+    sums[y][x] = sum;
+    __syncthreads();
+    unsigned before = 0;
+    for (unsigned r = 0; r < y; ++r) before += sums[r][x];
+    for (unsigned t = first; t < last; t += 8) {
+        unsigned c[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) c[k] = t + k < last ? column[(size_t)(t + k) * kTileDigits] : 0u;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (t + k < last) column[(size_t)(t + k) * kTileDigits] = before;
+            before += c[k];
+        }
+    }
+    if (y == kRuns - 1) column[(size_t)a.tiles * kTileDigits] = before;
+}
+
 // Tiles, a pass: ranks within the tile, offset by the counts of the tiles before it and of the
 // smaller digits.
 template <bool FIRST>
@@ -299,7 +338,12 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortArgs a) 
     static_assert(kSortThreads == 2 * kTileDigits, "two lanes a digit");
     const unsigned digit = threadIdx.x & (kTileDigits - 1), half = threadIdx.x / kTileDigits;
     unsigned before_me = 0, all = 0;
-    if (digit < digits)
+    if (a.scanned) {
+        if (digit < digits && !half) {
+            before_me = a.table[(size_t)blockIdx.x * kTileDigits + digit];
+            all = a.table[(size_t)a.tiles * kTileDigits + digit];
+        }
+    } else if (digit < digits) {
         for (unsigned t0 = half; t0 < a.tiles; t0 += 32) {
             unsigned c[16];
 #pragma unroll
@@ -310,6 +354,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortArgs a) 
                 if (t0 + 2 * k < blockIdx.x) before_me += c[k];
             }
         }
+    }
     if (half) start[digit] = all, part[digit] = before_me;
     __syncthreads();
     if (!half) {
@@ -740,7 +785,6 @@ int launch_lookup(const ContextView& c, const ngh_embedding_spec* s) {
     a.y = s->y;
     a.table_stride = s->table_stride;
     a.y_stride = s->y_stride;
-    a.rows = (unsigned)s->rows;
     a.vocab = (unsigned)s->vocab;
     a.width = (unsigned)s->width;
     a.chunks = (unsigned)((s->width + kVec - 1) / kVec);
@@ -749,10 +793,16 @@ int launch_lookup(const ContextView& c, const ngh_embedding_spec* s) {
     a.scale = s->scale;
     a.pad = s->pad_idx;
     const unsigned per_wg = kEmbBlock / a.lanes * kLookupRows;
-    const dim3 grid((a.rows + per_wg - 1) / per_wg);
-    if (vec) hipLaunchKernelGGL((embedding_kernel<TIn, TOut, kVec, false>), grid, dim3(kEmbBlock), 0, c.stream, a);
-    else hipLaunchKernelGGL((embedding_kernel<TIn, TOut, kVec, true>), grid, dim3(kEmbBlock), 0, c.stream, a);
-    NGH_HIP_TRY(hipGetLastError());
+    const int64_t slice = kMostThreads / kEmbBlock * per_wg;
+    for (int64_t first = 0; first < s->rows; first += slice) {
+        a.rows = (unsigned)std::min(slice, s->rows - first);
+        const dim3 grid((a.rows + per_wg - 1) / per_wg);
+        if (vec) hipLaunchKernelGGL((embedding_kernel<TIn, TOut, kVec, false>), grid, dim3(kEmbBlock), 0, c.stream, a);
+        else hipLaunchKernelGGL((embedding_kernel<TIn, TOut, kVec, true>), grid, dim3(kEmbBlock), 0, c.stream, a);
+        NGH_HIP_TRY(hipGetLastError());
+        a.tokens += slice;
+        a.y = (TOut*)a.y + slice * s->y_stride;
+    }
     return NGH_OK;
 }
 
@@ -791,7 +841,7 @@ GradPlan plan_grad(const ngh_embedding_spec* s, int cus) {
         g.places_a = at, at += room(4ull * n);
         g.keys_b = at, at += room(4ull * n);
         g.places_b = at, at += room(4ull * n);
-        g.tables = at, at += (size_t)g.tiles * kTileDigits * 4;
+        g.tables = at, at += (size_t)(g.tiles + 1) * kTileDigits * 4;
         g.parts = at, at += g.units > 1 ? (size_t)g.units * 2 * g.part_stride * 4 : 0;
     }
     g.bytes = at;
@@ -810,9 +860,7 @@ unsigned slabs_of(SumArgs& a, unsigned wgs, unsigned most, unsigned parts) {
 template <class TIn, class TOut, bool RAGGED>
 int launch_sums(const ContextView& c, SumArgs a, unsigned col_blocks) {
     constexpr int kVec = 16 / sizeof(TIn);
-    const unsigned long long jobs = (unsigned long long)a.units * col_blocks;
-    if (jobs >= (1ull << 31)) return report(NGH_E_UNSUPPORTED, "ngh_embedding_grad: grid too large");
-    a.workers = (unsigned)((jobs + 3) / 4);
+    a.workers = (a.units * col_blocks + 3) / 4;
     const unsigned grid = a.workers + slabs_of(a, 16 * c.cus, 64, kEmbBlock / 64);
     if (a.accumulate) hipLaunchKernelGGL((embedding_sum_kernel<TIn, TOut, kVec, RAGGED, true>), dim3(grid), dim3(kEmbBlock), 0, c.stream, a, col_blocks);
     else hipLaunchKernelGGL((embedding_sum_kernel<TIn, TOut, kVec, RAGGED, false>), dim3(grid), dim3(kEmbBlock), 0, c.stream, a, col_blocks);
@@ -894,6 +942,8 @@ int ngh_embedding_grad(ngh_context* ctx, const ngh_embedding_spec* spec) {
     if (spec->rows == 0 && spec->accumulate) return NGH_OK;
     const ContextView c = view_of(ctx);
     const GradPlan g = plan_grad(spec, c.cus);
+    if (!g.few && (long long)g.units * g.col_blocks >= kMostThreads / (kMergeWaves * 64))
+        return report(NGH_E_UNSUPPORTED, "ngh_embedding_grad: %lld rows of %lld elements", (long long)spec->rows, (long long)spec->width);
     if (spec->workspace_bytes < g.bytes || (g.bytes && !spec->workspace))
         return report(NGH_E_INVALID, "ngh_embedding_grad: workspace of %zu bytes, %zu needed", spec->workspace_bytes, g.bytes);
     if ((uintptr_t)spec->workspace % 16) return report(NGH_E_INVALID, "ngh_embedding_grad: misaligned workspace");
@@ -947,6 +997,7 @@ int ngh_embedding_grad(ngh_context* ctx, const ngh_embedding_spec* spec) {
         }
     } else if (!g.few) {
         const int digit = (g.bits + g.passes - 1) / g.passes;
+        s.scanned = g.tiles > (unsigned)kTilesUnscanned;
         for (int p = 0; p < g.passes; ++p) {
             s.shift = p * digit;
             s.bits = std::min(digit, g.bits - s.shift);
@@ -955,13 +1006,11 @@ int ngh_embedding_grad(ngh_context* ctx, const ngh_embedding_spec* spec) {
             s.place_out = (unsigned*)(ws + (a_out ? g.places_a : g.places_b));
             s.key_in = (const unsigned*)(ws + (a_out ? g.keys_b : g.keys_a));
             s.place_in = (const unsigned*)(ws + (a_out ? g.places_b : g.places_a));
-            if (p == 0) {
-                NGH_HIP_TRY(launch_sort(sort_count_kernel<true>, g.tiles, kSortThreads));
-                NGH_HIP_TRY(launch_sort(sort_scatter_kernel<true>, g.tiles, kSortThreads));
-            } else {
-                NGH_HIP_TRY(launch_sort(sort_count_kernel<false>, g.tiles, kSortThreads));
-                NGH_HIP_TRY(launch_sort(sort_scatter_kernel<false>, g.tiles, kSortThreads));
-            }
+            if (p == 0) NGH_HIP_TRY(launch_sort(sort_count_kernel<true>, g.tiles, kSortThreads));
+            else NGH_HIP_TRY(launch_sort(sort_count_kernel<false>, g.tiles, kSortThreads));
+            if (s.scanned) NGH_HIP_TRY(launch_sort(sort_scan_kernel, kTileDigits / kScanDigits, kSortThreads));
+            if (p == 0) NGH_HIP_TRY(launch_sort(sort_scatter_kernel<true>, g.tiles, kSortThreads));
+            else NGH_HIP_TRY(launch_sort(sort_scatter_kernel<false>, g.tiles, kSortThreads));
         }
     }
     SumArgs a{};

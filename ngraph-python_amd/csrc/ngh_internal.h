@@ -41,8 +41,13 @@ private:
 
 // Bytes a view of `rows` rows of `width` elements, `stride` elements apart, spans.
 inline unsigned long long span_bytes(int64_t rows, int64_t width, int64_t stride, int itemsize) {
-    return rows <= 0 || width <= 0 ? 0 : (unsigned long long)((rows - 1) * stride + width) * itemsize;
+    if (rows <= 0 || width <= 0) return 0;
+    const __int128 bytes = ((__int128)(rows - 1) * stride + width) * itemsize;
+    return bytes < (__int128)1 << 62 ? (unsigned long long)bytes : 1ull << 62;
 }
+
+// A grid has fewer than 2^32 threads; calls over more rows than that are launched in slices.
+constexpr long long kMostThreads = 1LL << 31;
 
 inline bool spans_overlap(const void* a, unsigned long long an, const void* b, unsigned long long bn) {
     const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;

@@ -205,6 +205,25 @@ def test_gradient_of_many_places_and_a_table_of_more_than_27_bits_of_tokens(hip_
     np.testing.assert_array_equal(got, want.astype(f32))
 
 
+@pytest.mark.parametrize("n,vocab,kind", [(262145, 300, "zipf"), (600001, 70001, "zipf"), (400000, 70001, "one"), (524289, 2000000, "any")])
+def test_gradient_of_more_tiles_than_a_tile_adds_up(hip_runtime, n, vocab, kind):
+    """One, two and three digits with the counts of all tiles added by a launch of its own."""
+    rt, rs = hip_runtime, np.random.RandomState(n)
+    tokens = tokens_for(rs, n, vocab, kind)
+    values = rs.randint(-8, 9, (n, 2)).astype(f32)                       # whole numbers: any order adds up exactly
+    want = np.stack([np.bincount(tokens, weights=values[:, i].astype(f64), minlength=vocab) for i in (0, 1)], 1)
+    with Pool(rt) as pool:
+        dy, t, table = pool.rows((n, 2), "f32", values), pool.array(tokens), pool.rows((vocab, 2), "f32")
+        spec = rt.embedding_grad_spec(n, vocab, 2, t.ptr, dy.ptr, table.ptr)
+        spec.workspace_bytes = rt.embedding_grad_workspace(spec)
+        work = pool.bytes(spec.workspace_bytes)
+        rt.memset32(work.ptr, 0xffffffff, spec.workspace_bytes // 4)
+        spec.workspace = work.ptr
+        rt.embedding_grad(spec)
+        got = table.get()
+    np.testing.assert_array_equal(got, want.astype(f32))
+
+
 def test_recorded_calls_replay_with_new_tokens(hip_runtime):
     """Lookup and gradient in one graph, replayed between eager calls that share the workspace."""
     rt = hip_runtime

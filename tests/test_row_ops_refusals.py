@@ -69,6 +69,18 @@ def test_calls_without_a_context_are_refused():
     refused(lambda: calls.adamw_step(row_ops.AdamWPlan(None, 0, 32), 1), -1, "ctx is NULL")
 
 
+def test_gate_rows_beyond_any_number_of_rows_are_refused():
+    """(of no rows every number of them is a whole share)"""
+    refused(lambda: norm(gate_rows=1 << 32, rows=0), -1, "gate_rows")
+    refused(lambda: norm(True, gate_rows=1 << 32, rows=0), -1, "gate_rows")
+    norm(True, gate_rows=7, rows=0)
+
+
+def test_spans_beyond_64_bits_are_seen_to_overlap():
+    far = dict(rows=(1 << 30) + 12, h_stride=(1 << 40) - 4, gate_rows=4)
+    refused(lambda: norm(**far), -1, "overlaps")
+
+
 def test_the_gradients_workspace_grows_with_what_it_holds():
     small = calls.embedding_grad_workspace(calls.embedding_grad_spec(10, 100, 64, 1, 2, 3))
     large = calls.embedding_grad_workspace(calls.embedding_grad_spec(100000, 100, 64, 1, 2, 3))
