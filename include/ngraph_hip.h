@@ -587,7 +587,8 @@ int  ngh_block_norm_grad_workspace(const ngh_block_norm_spec* spec, size_t* out_
  * so that a second moment only becomes 0 where it is below 1.5e-11 of the block's largest.  The
  * update uses the moments before they are rounded.  A block in which a moment is not finite gets
  * NaN for its scale: it shows in every element of the block from the next step on.  A tensor that is
- * written may overlap nothing else of the plan.                                                  */
+ * written may overlap nothing else of the plan.  Steps of one plan follow one another (on one stream,
+ * or ordered by the caller); a recorded graph reads the plan's memory as long as it is replayed.  */
 #define NGH_ADAMW_BLOCK 256
 typedef struct ngh_adamw_tensor {
     void*       param;               /* [n], param_dtype; updated in place                       */
@@ -619,7 +620,7 @@ int  ngh_validate_adamw(const ngh_adamw_tensor* tensors, int32_t n_tensors, int3
 int  ngh_adamw_plan_create(ngh_context* ctx, const ngh_adamw_tensor* tensors, int32_t n_tensors, int32_t param_dtype,
                            int32_t grad_dtype, int32_t copy_dtype, int32_t state_bits, ngh_adamw_plan** out);
 int  ngh_adamw_step(ngh_context* ctx, ngh_adamw_plan* plan, const ngh_adamw_hyper* hyper);
-int  ngh_adamw_plan_free(ngh_context* ctx, ngh_adamw_plan* plan);      /* waits for the stream */
+int  ngh_adamw_plan_free(ngh_context* ctx, ngh_adamw_plan* plan);      /* waits for the stream; not while a graph is recorded */
 /* n moments in 8 bits as fp32 and back (checkpoints); second: 0 the first moments, 1 the second.  */
 int  ngh_adamw_decode(ngh_context* ctx, float* dev_out, const void* dev_codes, const float* dev_scales, int64_t n,
                       int32_t second);

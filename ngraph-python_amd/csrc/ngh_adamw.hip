@@ -98,11 +98,12 @@ __device__ __forceinline__ float second_value(int q, float s) {
 // roots above, which take some 90 instructions an element for both; here approximate ones (v_rcp, v_sqrt: 1 ulp)
 // place the root within 7.5 * 2^-24 * 255 = 1.2e-4 steps of the exact chain's, so that only a root that
 // lies within 2^-12 of the border of two codes has to be worked out exactly, for the whole wavefront then (one
-// in eight blocks).  Scales too small for an approximate reciprocal take that way too.
+// in eight blocks).  Scales whose approximate reciprocal would be near overflow or below the normal numbers
+// (flushed to 0) take that way too.
 template <bool SECOND>
 __device__ __forceinline__ unsigned four_codes(const float (&x)[kPer], float s) {
     unsigned w = 0;
-    bool close = !(s >= 0x1p-100f);
+    bool close = !(s >= 0x1p-100f && s <= 0x1p100f);
     const float r = __builtin_amdgcn_rcpf(s);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
@@ -264,24 +265,27 @@ __global__ __launch_bounds__(kAdamBlock) void adamw_decode_kernel(float* out, co
     }
 }
 
-// A wavefront for each block of NGH_ADAMW_BLOCK values.
+// A wavefront for each block of NGH_ADAMW_BLOCK values (all of it makes the same turns).
 __global__ __launch_bounds__(kAdamBlock) void adamw_encode_kernel(unsigned char* codes, float* scales, const float* in, long long n, int second,
                                                                   int aligned) {
-    const long long at = ((long long)blockIdx.x * kAdamBlock + threadIdx.x) * kPer;
-    const int count = (int)max(0ll, min((long long)kPer, n - at));
-    const bool whole = aligned && count == kPer;
-    float v[kPer];
-    load_four(in, at, count, whole, v);
-    unsigned top = 0;
+    const long long step = (long long)gridDim.x * kAdamBlock * kPer;
+    for (long long base = ((long long)blockIdx.x * kAdamBlock + (threadIdx.x & ~63u)) * kPer; base < n; base += step) {
+        const long long at = base + (threadIdx.x & 63) * kPer;
+        const int count = (int)max(0ll, min((long long)kPer, n - at));
+        const bool whole = aligned && count == kPer;
+        float v[kPer];
+        load_four(in, at, count, whole, v);
+        unsigned top = 0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-    const float s = scale_of(top);
-    unsigned w = 0;
+        for (int j = 0; j < kPer; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+        const float s = scale_of(top);
+        unsigned w = 0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
-        w |= ((unsigned)(second ? second_code(v[j], s) : first_code(v[j], s)) & 255u) << (8 * j);
-    store_codes(codes, at, count, whole, w);
-    if ((threadIdx.x & 63) == 0 && count > 0) scales[at / NGH_ADAMW_BLOCK] = s;
+        for (int j = 0; j < kPer; ++j)
+            w |= ((unsigned)(second ? second_code(v[j], s) : first_code(v[j], s)) & 255u) << (8 * j);
+        store_codes(codes, at, count, whole, w);
+        if ((threadIdx.x & 63) == 0) scales[base / NGH_ADAMW_BLOCK] = s;
+    }
 }
 
 int size_of(int dtype) { return dtype == NGH_F32 ? 4 : (dtype == NGH_F16 || dtype == NGH_BF16) ? 2 : 0; }
@@ -367,7 +371,7 @@ int lay_out(const ngh_adamw_tensor* tensors, int32_t n_tensors, int cus, ngh_ada
     for (int i = 0; i < n_tensors; ++i) pieces += (tensors[i].n + kPiece - 1) / kPiece;
     plan.turns = pieces >= 4ll * kTurnsMany * cus ? kTurnsMany : kTurnsFew;
     const long long chunk = (long long)plan.turns * kPiece;
-    if (pieces >= (1LL << 31)) return report(NGH_E_UNSUPPORTED, "ngh_adamw: too many elements for one plan");
+    if (pieces / plan.turns + n_tensors >= 2 * kMostThreads / kAdamBlock) return report(NGH_E_UNSUPPORTED, "ngh_adamw: too many elements for one plan");
     for (int i = 0; i < n_tensors; ++i)
         for (long long c = 0; c * chunk < tensors[i].n; ++c) jobs.push_back(Job{i, (int)c});
     // nothing that is written may be anything else of the plan
@@ -537,6 +541,7 @@ int ngh_adamw_step(ngh_context* ctx, ngh_adamw_plan* plan, const ngh_adamw_hyper
 
 int ngh_adamw_plan_free(ngh_context* ctx, ngh_adamw_plan* plan) {
     if (!plan) return NGH_OK;
+    if (ctx && view_of(ctx).capturing) return report(NGH_E_INVALID, "ngh_adamw_plan_free: a graph is being recorded");
     if (ctx && plan->memory) (void)hipStreamSynchronize(view_of(ctx).stream);
     if (plan->memory) (void)hipFree(plan->memory);
     delete plan;
@@ -565,8 +570,8 @@ int ngh_adamw_encode(ngh_context* ctx, void* dev_codes, float* dev_scales, const
     if (!scope.ok()) return report(NGH_E_RUNTIME, "ngh_adamw_encode: the context's device cannot be made current");
     const long long wgs = (n + kAdamBlock * kPer - 1) / (kAdamBlock * kPer);
     const int aligned = (uintptr_t)dev_in % 16 == 0 && (uintptr_t)dev_codes % 4 == 0;
-    hipLaunchKernelGGL(adamw_encode_kernel, dim3((unsigned)wgs), dim3(kAdamBlock), 0, c.stream, (unsigned char*)dev_codes, dev_scales, dev_in,
-                       (long long)n, (int)second, aligned);
+    hipLaunchKernelGGL(adamw_encode_kernel, dim3((unsigned)std::min<long long>(wgs, 64ll * c.cus)), dim3(kAdamBlock), 0, c.stream,
+                       (unsigned char*)dev_codes, dev_scales, dev_in, (long long)n, (int)second, aligned);
     NGH_HIP_TRY(hipGetLastError());
     return NGH_OK;
 }

@@ -352,8 +352,10 @@ class HipRuntime(row_ops.OperatorCalls):
     # -- lifetime --------------------------------------------------------
     def close(self):
         if getattr(self, "ctx", None):
-            for plan in list(self._adamw_plans):
-                self.adamw_plan_free(plan)
+            for plan in self._adamw_plans:
+                self.lib.ngh_adamw_plan_free(self.ctx, plan.handle)
+                plan.handle = None
+            self._adamw_plans = []
             for ptr in list(self._allocs):
                 self.lib.ngh_free(self.ctx, ctypes.c_void_p(ptr))
             self._allocs.clear()

@@ -124,6 +124,8 @@ class OperatorCalls(object):
     def embedding_spec(self, rows, vocab, width, tokens, table, y, table_dtype=0, y_dtype=None, scale=1.0, pad_idx=-1,
                        table_stride=None, y_stride=None):
         """The spec of y[n, :] = scale * table[tokens[n], :]; strides default to the width."""
+        if not -2 ** 31 <= pad_idx < 2 ** 31:
+            raise ValueError("embedding: pad_idx %r is no int32" % (pad_idx,))
         s = ngh_embedding_spec()
         s.abi_version = self.abi_version
         s.rows, s.vocab, s.width = int(rows), int(vocab), int(width)
@@ -213,14 +215,16 @@ class OperatorCalls(object):
     def adamw_step(self, plan, step=0, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, dev_step=None, dev_lr=None,
                    dev_grad_scale=None):
         """One update of every tensor of the plan; `step` counts from 1 (or dev_step: an int32 on the device)."""
+        if not -2 ** 31 <= int(step) < 2 ** 31:
+            raise ValueError("adamw: step %r is no int32" % (step,))
         h = ngh_adamw_hyper(lr, beta1, beta2, eps, grad_scale, int(step), dev_step, dev_lr, dev_grad_scale)
         self._check(self.lib.ngh_adamw_step(self.ctx, plan.handle, ctypes.byref(h)))
 
     def adamw_plan_free(self, plan):
+        self._check(self.lib.ngh_adamw_plan_free(self.ctx, plan.handle))
+        plan.handle = None
         if plan in self._adamw_plans:
             self._adamw_plans.remove(plan)
-        handle, plan.handle = plan.handle, None
-        self._check(self.lib.ngh_adamw_plan_free(self.ctx, handle))
 
     def adamw_decode(self, out, codes, scales, n, second=False):
         """n first (second) moments held in 8 bits as fp32."""

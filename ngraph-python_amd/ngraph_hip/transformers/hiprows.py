@@ -116,6 +116,8 @@ class EmbeddingOp(og.TensorOp):
         table = _as_rows(table, width_axis)
         tokens = _dense(tokens)
         self.scale_factor, self.pad_idx = float(scale), -1 if pad_idx is None else int(pad_idx)
+        if not -2 ** 31 <= self.pad_idx < 2 ** 31:
+            raise ValueError("embedding: pad_idx {} is no int32".format(pad_idx))
         self.results = {}
         super(EmbeddingOp, self).__init__(args=(table, tokens), axes=tokens.axes + og.make_axes([width_axis]), dtype=table.dtype, **kwargs)
         self.deriv_handler = _Adjoint(self._adjoints)

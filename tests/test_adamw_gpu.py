@@ -188,6 +188,63 @@ def test_small_second_moments_and_any_eps(hip_runtime, bits, eps):
         model.free()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_moments_up_to_the_largest_numbers(hip_runtime, bits):
+    """Scales whose reciprocals are below the normal numbers."""
+    rt, rs = hip_runtime, np.random.RandomState(8)
+    with Pool(rt) as pool:
+        model = Model(pool, rt, [4000], ("f32", "f32"), bits)
+        t = model.tensors[0]
+        size = np.minimum(10.0 ** (24 + np.arange(4000) // 256), 3e38)
+        for name in ("m", "v"):
+            x = (np.clip(rs.normal(0, 0.4, 4000), -1, 1) * size).astype(f32)
+            x = np.abs(x) if name == "v" else x
+            if bits == 8:
+                q, scales = encode(x, name == "v")
+                t[name] = decode(q, scales, name == "v")
+                rt.memcpy_h2d(t["dev_" + name].ptr, q.view(np.uint8))
+                rt.memcpy_h2d(t["dev_%s_scale" % name].ptr, scales)
+            else:
+                t[name] = x
+                rt.memcpy_h2d(t["dev_" + name].ptr, x)
+        rt.adamw_step(model.plan, 9, **HYPER)
+        model.check_step(9)
+        model.free()
+
+
+def test_a_plan_is_not_freed_while_recording(hip_runtime):
+    from ngraph_hip.runtime import HipLibraryError
+    rt = hip_runtime
+    with Pool(rt) as pool:
+        model = Model(pool, rt, [500])
+        rt.graph_begin()
+        try:
+            with pytest.raises(HipLibraryError) as e:
+                model.free()
+        finally:
+            rt.graph_abandon()
+        assert "recorded" in str(e.value)
+        rt.adamw_step(model.plan, 1, **HYPER)
+        model.check_step(1)
+        model.free()
+
+
+@pytest.mark.parametrize("second", [False, True])
+def test_codes_of_more_blocks_than_a_launch_has_wavefronts(hip_runtime, second):
+    rt, n = hip_runtime, 64 * 256 * 1024 * 2 + 777
+    with Pool(rt) as pool:
+        x = np.tile(np.random.RandomState(3).normal(0, 1, 1 << 16).astype(f32), n // (1 << 16) + 1)[:n]
+        x = np.abs(x) if second else x
+        values, codes = pool.array(x), pool.array(np.zeros(n, np.uint8))
+        scales = pool.array(np.zeros((n + BLOCK - 1) // BLOCK, f32))
+        rt.adamw_encode(codes.ptr, scales.ptr, values.ptr, n, second)
+        q, s = encode(x, second)
+        np.testing.assert_array_equal(codes.get().view(q.dtype), q)
+        np.testing.assert_array_equal(scales.get(), s)
+        rt.adamw_decode(values.ptr, codes.ptr, scales.ptr, n, second)
+        np.testing.assert_array_equal(values.get(), decode(q, s, second))
+
+
 def test_a_plan_of_nothing(hip_runtime):
     plan = hip_runtime.adamw_plan([])
     hip_runtime.adamw_step(plan, 1)

@@ -346,3 +346,61 @@ def test_learning_rate_from_the_graph(hip_runtime):
             np.testing.assert_allclose(read(), at, atol=1e-5)
     finally:
         t.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("param", [f32, np.float16])
+def test_a_step_of_half_precision_tensors(hip_runtime, param):
+    """fp16 table, stream and gradients.  A result is rounded once (2^-11).  The gradients are taken at the stored
+    stream, each of whose values is off by 2^-11 of itself, at most 4 standard deviations here, and meets three
+    terms of the norm's Jacobian: 12 * 2^-11 of the largest gradient, the rows' own rounding and that of their sum
+    making it 16 (the gains' sums over 30 rows: of the sum of the largest terms)."""
+    f16, half = np.dtype(np.float16), 2.0 ** -11
+    V, F, T, N = axes(V=11, F=24, T=5, N=6)
+    rs = np.random.RandomState(2)
+    tv, wv = rs.normal(0, 1, (11, 24)).astype(f16), rs.normal(1, 0.2, 24).astype(f16).astype(param)
+    cv, tk = rs.normal(0, 1, (6, 5, 24)).astype(f16), rs.randint(0, 11, (6, 5)).astype(np.int32)
+    table, w = ng.variable([V, F], initial_value=tv, dtype=f16), ng.variable([F], initial_value=wv, dtype=np.dtype(param))
+    tokens, c = ng.placeholder([N, T], dtype=i32), ng.placeholder([N, T, F], dtype=f16)
+    x = ng.embedding(table, tokens, scale=2.0)
+    y, h = ng.block_norm(x, c, gain=w, kind="layer")
+    cost = ng.sum(y * c, out_axes=())
+    dtable, dw = ng.deriv(cost, table), ng.deriv(cost, w)
+    update = hiprows.AdamWOp([table], [dtable], lr=0.125, weight_decay=[0.0])
+    t = transformer()
+    try:
+        step = t.computation([y, h, dtable, dw, update], tokens, c)
+        read = t.computation(table)
+        got = [np.array(a) for a in step(tk, cv)[:4]]
+        after = np.array(read())
+    finally:
+        t.close()
+    t64, w64, c64 = tv.astype(f64), wv.astype(f64), cv.astype(f64)
+    h64 = 2.0 * t64[tk] + c64
+    y64 = norm64(h64, "layer") * w64
+    m = h64 - h64.mean(-1, keepdims=True)
+    dev = np.sqrt((m * m).mean(-1, keepdims=True) + 1e-5)
+    dz = c64 * w64
+    dx = dz / dev - m * (dz * m).mean(-1, keepdims=True) / dev ** 3 - (dz / dev).mean(-1, keepdims=True)
+    want = np.zeros((11, 24))
+    np.add.at(want, tk, 2.0 * dx)
+    size = np.zeros((11, 24))
+    np.add.at(size, tk, np.full(dx.shape, 2.0 * np.abs(dx).max()))
+    np.testing.assert_allclose(got[0], y64, rtol=half, atol=1e-5)
+    np.testing.assert_allclose(got[1], h64, rtol=half, atol=1e-6)
+    assert (np.abs(got[2] - want) <= 16 * half * size).all()
+    terms = np.abs(c64 * norm64(h64, "layer"))
+    assert np.abs(got[3] - (c64 * norm64(h64, "layer")).sum((0, 1))).max() <= 16 * half * 30 * terms.max()
+    # the first step is lr * sign(g), off by eps / |g| of it, and rounded to fp16
+    sure = np.abs(want) > np.maximum(16 * half * size, 1e-3)
+    assert sure.any()
+    stepped = t64 - 0.125 * np.sign(want)
+    assert (np.abs(after - stepped) <= half * np.abs(stepped) + 0.125 * 1e-4)[sure].all()
+
+
+def test_numbers_that_do_not_fit_are_refused():
+    V, F, N = axes(V=10, F=8, N=5)
+    table, tokens = ng.placeholder([V, F]), ng.placeholder([N], dtype=i32)
+    for pad in (2 ** 31, -2 ** 31 - 1):
+        with pytest.raises(ValueError):
+            ng.embedding(table, tokens, pad_idx=pad)
