@@ -250,10 +250,10 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4))) vo
         float h[C][VEC], t[C][VEC], b[C][VEC], d[C][VEC];
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            to_float<T, VEC, RAGGED>(rh[c], in[c], h[c]);
-            to_float<T, VEC, RAGGED>(rt[c], in[c], t[c]);
-            to_float<T, VEC, RAGGED>(rb[c], in[c], b[c]);
-            to_float<T, VEC, RAGGED>(rd[c], in[c], d[c]);
+            take_piece<T, VEC, RAGGED>(rh[c], in[c], h[c]);
+            take_piece<T, VEC, RAGGED>(rt[c], in[c], t[c]);
+            take_piece<T, VEC, RAGGED>(rb[c], in[c], b[c]);
+            take_piece<T, VEC, RAGGED>(rd[c], in[c], d[c]);
         }
         fetch(n + 1, n + 1 < last);
         float brs = 1.0f;

@@ -75,6 +75,19 @@ __device__ __forceinline__ void to_float(const typename VecOf<T, V>::type& v, in
     for (int i = 0; i < V; ++i) out[i] = !RAGGED || i < count ? (float)v[i] : 0.0f;
 }
 
+// The same, worked out here: loads that follow stay behind it and may fill v again.  Left to itself the compiler uses
+// v only where the floats are needed, behind the loads of the next piece, and, since those are conditional,
+// waits for them too, so that nothing is in flight meanwhile.
+template <class T, int V, bool RAGGED>
+__device__ __forceinline__ void take_piece(const typename VecOf<T, V>::type& v, int count, float (&out)[V]) {
+    to_float<T, V, RAGGED>(v, count, out);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        if constexpr (sizeof(T) == 4 && !RAGGED) asm volatile("v_mov_b32 %0, %1" : "=v"(out[i]) : "v"((float)v[i]) : "memory");
+        else asm volatile("" : "+v"(out[i])::"memory");
+    }
+}
+
 template <class T, int V, bool RAGGED>
 __device__ __forceinline__ void load_piece(const T* p, int count, bool inside, float (&out)[V]) {
     to_float<T, V, RAGGED>(load_raw<T, V, RAGGED>(p, count, inside), count, out);
