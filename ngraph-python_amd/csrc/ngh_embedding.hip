@@ -565,23 +565,33 @@ __global__ __launch_bounds__(kFewWaves * 64) void embedding_few_kernel(SumArgs a
     __shared__ float sums[kFewWaves][64 * VEC];
     __shared__ unsigned counts[kFewWaves], token_of[kFewWaves];
     const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // (all tokens in flight at once: the last one again behind the end)
+    constexpr int kEach = kFew / (kFewWaves * 64);
+    unsigned token_key[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) token_key[k] = a.n ? (unsigned)tokens[min(threadIdx.x + k * kFewWaves * 64, a.n - 1)] : ~0u;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) token_key[k] = key_of((int)token_key[k], a.vocab, pad);
     if (blockIdx.x >= a.workers) {
         unsigned char* occurs = reinterpret_cast<unsigned char*>(found);
         static_assert(sizeof(found) >= kFewRows, "a slab's marks fit");
         const unsigned r0 = (blockIdx.x - a.workers) * a.slab, r1 = min(a.vocab, r0 + a.slab);
         for (unsigned r = threadIdx.x; r < r1 - r0; r += kFewWaves * 64) occurs[r] = 0;
         __syncthreads();
-        for (unsigned i = threadIdx.x; i < a.n; i += kFewWaves * 64) {
-            const unsigned key = key_of(tokens[i], a.vocab, pad);
-            if (key >= r0 && key < r1) occurs[key - r0] = 1;
-        }
+#pragma unroll
+        for (int k = 0; k < kEach; ++k)
+            if (token_key[k] >= r0 && token_key[k] < r1) occurs[token_key[k] - r0] = 1;
         __syncthreads();
         const unsigned each = (r1 - r0 + kFewWaves - 1) / kFewWaves, last = min(r1, r0 + (wave + 1) * each);
         for (unsigned r = r0 + wave * each; r < last; r += 64)
             clear_rows<TOut, RAGGED>(a, r, r + lane < last && !occurs[r + lane - r0]);
         return;
     }
-    for (unsigned i = threadIdx.x; i < kFew; i += kFewWaves * 64) keys[i] = i < a.n ? key_of(tokens[i], a.vocab, pad) : ~0u;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const unsigned i = threadIdx.x + k * kFewWaves * 64;
+        keys[i] = i < a.n ? token_key[k] : ~0u;
+    }
     __syncthreads();
     const unsigned group = blockIdx.x / col_parts, cp = blockIdx.x - group * col_parts;
     // (frequent tokens have their first places near the front: a workgroup's places lie far apart)
