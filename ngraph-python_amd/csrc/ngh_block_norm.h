@@ -43,15 +43,17 @@ struct NormArgs {
 constexpr int kVecGain = 1, kVecBias = 2, kVecPostGain = 4, kVecPostBias = 8, kVecGate = 16;
 
 // VEC elements of a gain, bias or gate; `other` where there is none.
-template <class T, int VEC, bool RAGGED>
-__device__ __forceinline__ void load_param(const void* p, long long at, int count, bool f32, float other, float (&out)[VEC]) {
+template <class T, int VEC, bool RAGGED, bool FORWARD>
+__device__ __forceinline__ void load_param(const void* p, long long at, unsigned col, int count, bool f32, float other, float (&out)[VEC]) {
     if (!p) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) out[i] = other;
     } else if (f32) {
         load_piece<float, VEC, RAGGED>((const float*)p + at, count, false, out);
     } else {
-        load_piece<T, VEC, RAGGED>((const T*)p + at, count, false, out);
+        // (in the forward pass, where every row loads them; vectors in fp32, and the backward pass, lost by it)
+        if constexpr (RAGGED && FORWARD) load_end<T, VEC>((const T*)p + at, count, col > 0, out);
+        else load_piece<T, VEC, RAGGED>((const T*)p + at, count, false, out);
     }
 }
 
@@ -77,19 +79,32 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a) {
     }
     // Gains, biases and gate are asked for with the rows rather than behind the reductions, where each costs its
     // latency again: 16384 rows of 4096 bf16 elements 98 us, 103 then.
+    // Not where a workgroup has more than 512 lanes: without their registers two such workgroups fit a compute unit
+    // (8192 rows of 8192 bf16 elements 145 us, 102 so); nor on any boundary, where their masks wait for them
+    // ([16384, 4095] 152 us, 147 so).
+    constexpr bool kEarly = THREADS <= 512 && !RAGGED;
     float p[C][VEC], q[C][VEC], g[C][VEC], w[C][VEC], z[C][VEC];
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
+    auto load_post = [&](int c) {
         const unsigned col = (c * lanes + lane) * VEC;
-        if (!in[c]) continue;
-        if (a.post) {
-            load_param<T, VEC, RAGGED>(a.post_gain, col, in[c], a.param_f32, 1.0f, p[c]);
-            load_param<T, VEC, RAGGED>(a.post_bias, col, in[c], a.param_f32, 0.0f, q[c]);
-        }
-        load_param<T, VEC, RAGGED>(a.gate, a.gate ? (long long)(n / a.gate_rows) * a.gate_stride + col : 0, in[c], a.param_f32, 1.0f, g[c]);
-        if (a.y) {
-            load_param<T, VEC, RAGGED>(a.gain, col, in[c], a.param_f32, 1.0f, w[c]);
-            load_param<T, VEC, RAGGED>(a.bias, col, in[c], a.param_f32, 0.0f, z[c]);
+        load_param<T, VEC, RAGGED, true>(a.post_gain, col, col, in[c], a.param_f32, 1.0f, p[c]);
+        load_param<T, VEC, RAGGED, true>(a.post_bias, col, col, in[c], a.param_f32, 0.0f, q[c]);
+    };
+    auto load_gate = [&](int c) {
+        const unsigned col = (c * lanes + lane) * VEC;
+        load_param<T, VEC, RAGGED, true>(a.gate, a.gate ? (long long)(n / a.gate_rows) * a.gate_stride + col : 0, col, in[c], a.param_f32, 1.0f, g[c]);
+    };
+    auto load_gain = [&](int c) {
+        const unsigned col = (c * lanes + lane) * VEC;
+        load_param<T, VEC, RAGGED, true>(a.gain, col, col, in[c], a.param_f32, 1.0f, w[c]);
+        load_param<T, VEC, RAGGED, true>(a.bias, col, col, in[c], a.param_f32, 0.0f, z[c]);
+    };
+    if constexpr (kEarly) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if (!in[c]) continue;
+            if (a.post) load_post(c);
+            load_gate(c);
+            if (a.y) load_gain(c);
         }
     }
     float v[C][VEC], x[C][VEC];
@@ -122,6 +137,7 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             if (in[c]) {
+                if constexpr (!kEarly) load_post(c);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) v[c][i] = v[c][i] * r * p[c][i] + q[c][i];
             }
@@ -131,6 +147,7 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a) {
     for (int c = 0; c < C; ++c) {
         const unsigned col = (c * lanes + lane) * VEC;
         if (in[c]) {
+            if constexpr (!kEarly) load_gate(c);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) v[c][i] = a.alpha * x[c][i] + v[c][i] * g[c][i];
             if (a.h) store_piece<T, VEC, RAGGED>((T*)a.h + (long long)n * a.h_stride + col, in[c], v[c]);
@@ -161,6 +178,7 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a) {
     for (int c = 0; c < C; ++c) {
         const unsigned col = (c * lanes + lane) * VEC;
         if (in[c]) {
+            if constexpr (!kEarly) load_gain(c);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) v[c][i] = v[c][i] * r * w[c][i] + z[c][i];
             store_piece<T, VEC, RAGGED>((T*)a.y + (long long)n * a.y_stride + col, in[c], v[c]);
@@ -225,11 +243,11 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4))) vo
             if (!in[c]) continue;
             const unsigned col = (c * lanes + lane) * VEC;
             float w[VEC], p[VEC], q[VEC], g[VEC];
-            if (a.in_lds & kVecGain) load_param<T, VEC, RAGGED>(a.gain, col, in[c], a.param_f32, 1.0f, w);
-            if (a.in_lds & kVecPostGain) load_param<T, VEC, RAGGED>(a.post_gain, col, in[c], a.param_f32, 1.0f, p);
-            if (a.in_lds & kVecPostBias) load_param<T, VEC, RAGGED>(a.post_bias, col, in[c], a.param_f32, 0.0f, q);
+            if (a.in_lds & kVecGain) load_param<T, VEC, RAGGED, false>(a.gain, col, col, in[c], a.param_f32, 1.0f, w);
+            if (a.in_lds & kVecPostGain) load_param<T, VEC, RAGGED, false>(a.post_gain, col, col, in[c], a.param_f32, 1.0f, p);
+            if (a.in_lds & kVecPostBias) load_param<T, VEC, RAGGED, false>(a.post_bias, col, col, in[c], a.param_f32, 0.0f, q);
             if (a.in_lds & kVecGate)                     // (a part's rows share a gate row where the gate is copied)
-                load_param<T, VEC, RAGGED>(a.gate, (long long)(part_first / a.gate_rows) * a.gate_stride + col, in[c], a.param_f32, 1.0f, g);
+                load_param<T, VEC, RAGGED, false>(a.gate, (long long)(part_first / a.gate_rows) * a.gate_stride + col, col, in[c], a.param_f32, 1.0f, g);
             if (a.in_lds & kVecGain) store_from_float<float, VEC>(lds + col, w);
             if (a.in_lds & kVecPostGain) store_from_float<float, VEC>(lds_post_gain + col, p);
             if (a.in_lds & kVecPostBias) store_from_float<float, VEC>(lds_post_bias + col, q);
@@ -238,7 +256,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(4))) vo
     }
     auto param = [&](int bit, const float* copy, const void* p, long long at, unsigned col, int count, float other, float (&out)[VEC]) {
         if (a.in_lds & bit) load_as_float<float, VEC>(copy + col, out);
-        else load_param<T, VEC, RAGGED>(p, at, count, a.param_f32, other, out);
+        else load_param<T, VEC, RAGGED, false>(p, at, col, count, a.param_f32, other, out);
     };
     // (every group of lanes of a workgroup makes the same number of turns)
     for (unsigned turn = 0; turn < a.per_group; ++turn) {

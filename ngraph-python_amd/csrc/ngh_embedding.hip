@@ -417,7 +417,7 @@ __device__ __forceinline__ void finish_row(const SumArgs& a, unsigned token, uns
     TOut* to = (TOut*)a.table + (long long)token * a.table_stride + col;
     float v[VEC];
     if (a.accumulate) {
-        load_piece<TOut, VEC, RAGGED>(to, in, false, v);
+        load_piece<TOut, VEC, RAGGED>(to, in, token + 1 < a.vocab && a.width >= VEC, v);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[i] += a.scale * acc[i];
     } else {
@@ -506,7 +506,7 @@ __global__ __launch_bounds__(kEmbBlock) void embedding_sum_kernel(SumArgs a, uns
                 to[k] = load_raw<TIn, VEC, RAGGED>(dy + (long long)place * a.dy_stride, in, place + 1 < a.n && a.width >= VEC);
                 if constexpr (ADD) {
                     const unsigned key = key_at(i + k);
-                    if (key != key_at(i + k + 1)) old[k] = load_raw<TOut, VEC, RAGGED>(table + (long long)key * a.table_stride, in, false);
+                    if (key != key_at(i + k + 1)) old[k] = load_raw<TOut, VEC, RAGGED>(table + (long long)key * a.table_stride, in, key + 1 < a.vocab && a.width >= VEC);
                 }
             }
         }

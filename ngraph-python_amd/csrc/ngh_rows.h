@@ -93,6 +93,29 @@ __device__ __forceinline__ void load_piece(const T* p, int count, bool inside, f
     to_float<T, V, RAGGED>(load_raw<T, V, RAGGED>(p, count, inside), count, out);
 }
 
+// The piece of a vector on any boundary, zeros behind its end.  Nothing may be read behind the vector: its last
+// piece is loaded from V elements before the end where there are as many (`behind_another`: it is not the first),
+// and shifted (norms of [16384, 4095] with gains in bf16: 169 us, 146 so).
+template <class T, int V>
+__device__ __forceinline__ void load_end(const T* p, int count, bool behind_another, float (&out)[V]) {
+    if (count == V) {
+        load_piece<T, V, true>(p, V, false, out);
+    } else if (count > 0 && behind_another) {
+        const int shift = V - count;
+        load_piece<T, V, true>(p - shift, V, false, out);
+#pragma unroll
+        for (int bit = V / 2; bit > 0; bit /= 2) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float further = i + bit < V ? out[i + bit < V ? i + bit : 0] : 0.0f;
+                out[i] = shift & bit ? further : out[i];
+            }
+        }
+    } else {
+        load_piece<T, V, true>(p, count, false, out);
+    }
+}
+
 template <class T, int V, bool RAGGED>
 __device__ __forceinline__ void store_piece(T* p, int count, const float (&in)[V]) {
     if (RAGGED ? count == V : count > 0) {
