@@ -77,7 +77,7 @@ __device__ __forceinline__ void to_float(const typename VecOf<T, V>::type& v, in
 
 // The same, worked out here: loads that follow stay behind it and may fill v again.  Left to itself the compiler uses
 // v only where the floats are needed, behind the loads of the next piece, and, since those are conditional,
-// waits for them too, so that nothing is in flight meanwhile.
+// waits for them too, so that nothing is in flight meanwhile (the same rows: 104 us, 92 so).
 template <class T, int V, bool RAGGED>
 __device__ __forceinline__ void take_piece(const typename VecOf<T, V>::type& v, int count, float (&out)[V]) {
     to_float<T, V, RAGGED>(v, count, out);
