@@ -10,6 +10,11 @@ optimizer.py:446-470); those compositions stay as they are, these ops stand besi
 An op here has one tensor as its result like any other; what its kernel writes besides (the stream
 after a block, the gradients of gains) are `RowResultOp`s that depend on it: their buffers are
 filled by that kernel, and one that nothing uses is not computed.
+
+The kernels take an operand as an address and at most one stride.  What an operand's description is
+shows only behind the graph passes, which turn 1 * x, x + 0 and folded constants into views: an
+operand that they may replace stands behind a `RowLayoutOp`, which `RowLayoutPass`, the last pass,
+resolves to the operand itself or to a copy of it.  Every kernel checks what it is bound to.
 """
 from __future__ import division
 
@@ -18,6 +23,7 @@ import numpy as np
 from ngraph_hip.op_graph import op_graph as og
 from ngraph_hip.transformers.hipdevice import _td
 from ngraph_hip.transformers.hiplowering import HipKernel, og_unsupported
+from ngraph_hip.transformers.passes.passes import PeepholeGraphPass
 
 F32, F16, I32 = np.dtype(np.float32), np.dtype(np.float16), np.dtype(np.int32)
 STATE_BLOCK = 256                       # elements that share a scale in 8-bit optimiser states
@@ -51,19 +57,56 @@ def rows_of(td, width_axis):
     return rows, width_axis.length, row_stride if rows > 1 else width_axis.length
 
 
+def _fits(td, dtype, width_axis):
+    """Whether a row kernel can take a tensor of this description as `dtype` operand: rows along width_axis, or
+    with None elements in C order."""
+    return td.dtype == dtype and (td.c_contiguous if width_axis is None else rows_of(td, width_axis) is not None)
+
+
+class RowLayoutOp(og.TensorOp):
+    """x as a row kernel takes it (`_fits`); in the graph until RowLayoutPass has seen what the other passes made
+    of x."""
+
+    def __init__(self, x, width_axis, **kwargs):
+        super(RowLayoutOp, self).__init__(args=(x,), axes=x.axes, dtype=x.dtype, **kwargs)
+        self.width_axis = width_axis
+        self.deriv_handler = _Adjoint(lambda add_delta, adjoints, delta: add_delta(adjoints, self.args[0], delta))
+
+
+class RowLayoutPass(PeepholeGraphPass):
+    """Resolves every RowLayoutOp; has to be the last pass."""
+
+    def visit(self, op, *args):
+        if isinstance(op, RowLayoutOp):
+            x, = args
+            td = _td(x)
+            if _fits(td, op.dtype, op.width_axis):
+                self.replace_op(op, x)
+            elif td.dtype == op.dtype:
+                self.replace_op(op, og.ContiguousOp(x))
+            else:
+                # (x16 * 1.0 has dtype float32 and becomes x16)
+                self.replace_op(op, _copied(x, op.axes, op.dtype))
+
+
+def _laid_out(x, width_axis):
+    # (no pass replaces the read of a tensor with storage of its own)
+    x = og.as_op(x)
+    return x if isinstance(x, og.TensorValueOp) and _fits(_td(x), x.dtype, width_axis) else RowLayoutOp(x, width_axis)
+
+
 def _as_rows(x, width_axis):
     """x with width_axis last and rows as rows_of wants them, by a device copy if there is no other way."""
     x = og.as_op(x)
     if x.axes[len(x.axes) - 1] != width_axis:
         others = [a for a in x.axes if a != width_axis]
         x = og.axes_with_order(x, og.make_axes(others + [width_axis]))
-    return x if rows_of(_td(x), width_axis) is not None else og.ContiguousOp(x)
+    return _laid_out(x, width_axis)
 
 
 def _dense(x):
     """x in C order, by a device copy if its view is not."""
-    x = og.as_op(x)
-    return x if _td(x).c_contiguous else og.ContiguousOp(x)
+    return _laid_out(x, None)
 
 
 def _check_dtype(op, allowed, what):
@@ -74,9 +117,11 @@ def _check_dtype(op, allowed, what):
 def _cast(x, dtype):
     """x as `dtype` (a device copy where it is another)."""
     x = og.as_op(x)
-    if x.dtype == dtype:
-        return x
-    copy = og.temporary(axes=x.axes, dtype=dtype)
+    return x if x.dtype == dtype else _copied(x, x.axes, dtype)
+
+
+def _copied(x, axes, dtype):
+    copy = og.temporary(axes=axes, dtype=dtype)
     return og.sequential([og.AssignOp(copy, x), copy])
 
 
@@ -286,6 +331,7 @@ class AdamWOp(og.Op):
             if len(kinds) > 1:
                 raise ValueError("AdamW: %s of several dtypes; use an op for each" % what)
         self.variables, self.n = list(variables), len(variables)
+        self.grad_dtype = args[0].dtype if args else F32
         self.beta_1, self.beta_2, self.epsilon = float(beta_1), float(beta_2), float(epsilon)
         self.weight_decay, self.state_bits, self.grad_scale = [float(w) for w in weight_decay], state_bits, float(grad_scale)
         self.lr = lr if isinstance(lr, og.Op) else float(lr)
@@ -296,7 +342,7 @@ class AdamWOp(og.Op):
                 if not s.is_scalar or s.dtype != F32:
                     raise ValueError("AdamW: %s is a float32 scalar, got %s %s" % (name, s.axes, s.dtype))
                 self.scalar_names.append(name)
-                args.append(s)
+                args.append(_dense(s))
         self.step = og.persistent_tensor(axes=(), dtype=I32, initial_value=0)
         self.m, self.v, self.m_scale, self.v_scale = [], [], [], []
         for var in variables:
@@ -344,12 +390,23 @@ class RowKernel(HipKernel):
     def code(self, dtype):
         return self.transformer.ngh_dtype(dtype)
 
-    def rows(self, op, width_axis):
+    def checked(self, op, axes, dtype, width_axis=None):
+        """The description of an operand, after checking that the kernel can take it."""
+        td = _td(op.forwarded)
+        if not _fits(td, dtype, width_axis) or td.axes.lengths != og.make_axes(axes).lengths:
+            raise og_unsupported("%s: operand %s is %s with strides %s, %s" % (type(self.op).__name__, op, td.axes, tuple(td.full_strides), td.dtype))
+        return td
+
+    def rows(self, op, axes, dtype):
         """(address, rows, row stride) of a row operand."""
-        layout = rows_of(_td(op.forwarded), width_axis)
-        if layout is None:
-            raise og_unsupported("%s: operand %s lost its row layout" % (type(self.op).__name__, op))
+        width_axis = axes[len(axes) - 1]
+        layout = rows_of(self.checked(op, axes, dtype, width_axis), width_axis)
         return self.view(op).ptr, layout[0], layout[2]
+
+    def dense(self, op, axes, dtype):
+        """The address of an operand whose elements follow one another."""
+        self.checked(op, axes, dtype)
+        return self.view(op).ptr
 
     def results(self):
         """The op's further results that the transformer's computations hold: {name: op}."""
@@ -375,10 +432,11 @@ class EmbeddingKernel(RowKernel):
     def bind_buffers(self):
         table, tokens = (a.forwarded for a in self.op.args)
         width = self.op.axes[len(self.op.axes) - 1]
-        at, vocab, stride = self.rows(table, width)
-        y, n, y_stride = self.rows(self.op, width)
-        self.spec = self.transformer.runtime.embedding_spec(n, vocab, width.length, self.view(tokens).ptr, at, y, self.code(table.dtype),
-                                                            None, self.op.scale_factor, self.op.pad_idx, stride, y_stride)
+        at, vocab, stride = self.rows(table, table.axes, self.op.dtype)
+        y, n, y_stride = self.rows(self.op, self.op.axes, self.op.dtype)
+        self.spec = self.transformer.runtime.embedding_spec(
+            n, vocab, width.length, self.dense(tokens, list(self.op.axes)[:-1], I32), at, y, self.code(self.op.dtype), None,
+            self.op.scale_factor, self.op.pad_idx, stride, y_stride)
         super(EmbeddingKernel, self).bind_buffers()
 
     def execute(self):
@@ -392,10 +450,10 @@ class EmbeddingGradKernel(RowKernel):
         rt = self.transformer.runtime
         tokens, delta = (a.forwarded for a in self.op.args)
         width = self.op.axes[1]
-        at, vocab, stride = self.rows(self.op, width)
-        dy, n, dy_stride = self.rows(delta, width)
-        s = rt.embedding_grad_spec(n, vocab, width.length, self.view(tokens).ptr, dy, at, self.code(delta.dtype), None, self.op.scale_factor,
-                                   self.op.pad_idx, False, stride, dy_stride)
+        at, vocab, stride = self.rows(self.op, self.op.axes, self.op.dtype)
+        dy, n, dy_stride = self.rows(delta, list(tokens.axes) + [width], self.op.dtype)
+        s = rt.embedding_grad_spec(n, vocab, width.length, self.dense(tokens, tokens.axes, I32), dy, at, self.code(self.op.dtype), None,
+                                   self.op.scale_factor, self.op.pad_idx, False, stride, dy_stride)
         s.workspace_bytes = rt.embedding_grad_workspace(s)
         s.workspace = self.workspace(s.workspace_bytes)
         self.spec = s
@@ -411,9 +469,11 @@ def _norm_spec(kernel, norm, operands):
     fields = {}
     for name, op in operands.items():
         if name in ("gain", "bias", "post_gain", "post_bias", "dgain", "dbias", "dpost_gain", "dpost_bias"):
-            fields[name] = kernel.view(op).ptr
+            fields[name] = kernel.dense(op, [width], norm.param_dtype)
+        elif name in ("gate", "dgate"):
+            fields[name], _, fields[name + "_stride"] = kernel.rows(op, norm.operand("gate").axes, norm.param_dtype)
         else:
-            fields[name], _, fields[name + "_stride"] = kernel.rows(op, width)
+            fields[name], _, fields[name + "_stride"] = kernel.rows(op, norm.axes, norm.dtype)
     return kernel.transformer.runtime.block_norm_spec(
         norm.axes.size // width.length, width.length, norm.kind, kernel.code(norm.dtype), kernel.code(norm.param_dtype), norm.post_norm,
         norm.gate_rows if "gate" in operands else 0, norm.residual_scale, norm.eps, **fields)
@@ -479,20 +539,20 @@ class AdamWKernel(RowKernel):
 
     def bind_buffers(self):
         op, rt = self.op, self.transformer.runtime
-        at = lambda t: self.transformer.get_tensor_description_tensor_view(_td(t)).ptr               # noqa: E731
+        at = lambda t: self.dense(t, t.axes, t.dtype)                                                 # noqa: E731
         rows = []
         for i, var in enumerate(op.variables):
-            row = dict(param=at(var), grad=self.view(op.args[i]).ptr, m=at(op.m[i]), v=at(op.v[i]), n=var.axes.size,
+            row = dict(param=at(var), grad=self.dense(op.args[i], var.axes, op.grad_dtype), m=at(op.m[i]), v=at(op.v[i]), n=var.axes.size,
                        weight_decay=op.weight_decay[i])
             if op.state_bits == 8:
                 row.update(m_scale=at(op.m_scale[i]), v_scale=at(op.v_scale[i]))
             rows.append(row)
-        kinds = dict(param_dtype=self.code(op.variables[0].dtype), grad_dtype=self.code(op.args[0].forwarded.dtype)) if rows else {}
+        kinds = dict(param_dtype=self.code(op.variables[0].dtype), grad_dtype=self.code(op.grad_dtype)) if rows else {}
         self.plan = rt.adamw_plan(rows, state_bits=op.state_bits, **kinds)
         scalars = dict(zip(op.scalar_names, op.args[op.n:]))
         self.hyper = dict(lr=0.0 if "lr" in scalars else op.lr, beta1=op.beta_1, beta2=op.beta_2, eps=op.epsilon, grad_scale=op.grad_scale,
-                          dev_step=at(op.step), dev_lr=self.view(scalars["lr"]).ptr if "lr" in scalars else None,
-                          dev_grad_scale=self.view(scalars["clip"]).ptr if "clip" in scalars else None)
+                          dev_step=at(op.step), dev_lr=self.dense(scalars["lr"], (), F32) if "lr" in scalars else None,
+                          dev_grad_scale=self.dense(scalars["clip"], (), F32) if "clip" in scalars else None)
         super(AdamWKernel, self).bind_buffers()
 
     def execute(self):

@@ -44,7 +44,7 @@ from ngraph_hip.transformers.hipdevice import HipDeviceBufferStorage, HipDeviceT
 from ngraph_hip.transformers.hiplowering import (FusedKernel, CopyKernel, HipKernel, kernel_op_name,  # noqa: F401
                                                  is_fusable, iteration_axes, og_unsupported)
 from ngraph_hip.transformers.hipmoments import MomentsOp, MomentsFusionPass, MomentsKernel, moments_layout  # noqa: F401
-from ngraph_hip.transformers.hiprows import row_kernel
+from ngraph_hip.transformers.hiprows import RowLayoutPass, row_kernel
 from ngraph_hip.transformers.hipchains import ChainKernel, KernelRun  # noqa: F401
 from ngraph_hip.transformers.hipplanner import FusionPlanner
 
@@ -340,6 +340,7 @@ class HipTransformer(ComputationGraphTransformer):
         if fusion if fuse_moments is None else fuse_moments:
             self.graph_passes.append(MomentsFusionPass())
         self.graph_passes.append(ReductionLayoutPass(split=self.split_reductions))
+        self.graph_passes.append(RowLayoutPass())
 
     # -- dtype mapping ---------------------------------------------------------------------
     def ngh_dtype(self, dtype):
