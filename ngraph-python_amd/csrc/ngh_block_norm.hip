@@ -25,6 +25,7 @@ constexpr int kMostViews = 20;
 struct Views {
     View v[kMostViews];
     int n = 0;
+    int in_place = -1, over = -1;      // the output that may be the same view as an input, and that input
 };
 
 // Everything the call touches.
@@ -41,14 +42,18 @@ void views_of(const ngh_block_norm_spec* s, bool grad, Views& views) {
     add("post_bias", s->post_bias, 1, s->width, q, false);
     add("gate", s->gate, gates, s->gate_stride, q, false);
     add("b", s->b, s->rows, s->b_stride, e, false);
+    if (!grad && s->h) views.in_place = n;
     add("h", s->h, s->rows, s->h_stride, e, !grad);
     if (!grad) {
         add("bias", s->bias, 1, s->width, q, false);
+        if (s->x) views.over = n;
         add("x", s->x, s->rows, s->x_stride, e, false);
         add("y", s->y, s->rows, s->y_stride, e, true);
     } else {
         add("dy", s->dy, s->rows, s->dy_stride, e, false);
+        if (s->dh) views.over = n;
         add("dh", s->dh, s->rows, s->dh_stride, e, false);
+        if (s->dx) views.in_place = n;
         add("dx", s->dx, s->rows, s->dx_stride, e, true);
         add("db", s->db, s->rows, s->db_stride, e, true);
         add("dgain", s->dgain, 1, s->width, q, true);
@@ -112,9 +117,10 @@ int check(const ngh_block_norm_spec* s, bool grad, const char* what, Views& view
         for (int j = 0; j < n; ++j) {
             if (i == j || !v[i].written || (v[j].written && j < i)) continue;
             if (!spans_overlap(v[i].p, bytes(v[i]), v[j].p, bytes(v[j]))) continue;
-            // a row is read whole before it is written: the stream and its gradient may be updated in place
+            // a row is read whole before it is written: the stream and its gradient may be updated in place (these two
+            // views and no others, whatever else has their address)
             const bool same = v[i].p == v[j].p && (v[i].stride == v[j].stride || s->rows == 1);
-            if (same && ((v[i].p == s->h && v[j].p == s->x && !grad && v[j].p != s->b) || (grad && v[i].p == s->dx && v[j].p == s->dh))) continue;
+            if (same && i == views.in_place && j == views.over) continue;
             return report(NGH_E_INVALID, "%s: %s overlaps %s", what, v[i].name, v[j].name);
         }
     return NGH_OK;

@@ -1,0 +1,48 @@
+"""What the header says of the operators over rows and parameters beyond single arguments: several operands that share
+memory, calls over nothing, counters, without a device where that is possible."""
+import ctypes
+
+import pytest
+
+from ngraph_hip.runtime import HipLibraryError, load_library, row_ops
+from ngraph_hip.runtime.hiplib import NGH_ABI_VERSION, _check
+
+
+class Calls(row_ops.OperatorCalls):
+    """The spec builders without a device."""
+    abi_version = NGH_ABI_VERSION
+
+    def __init__(self):
+        self.lib, self.ctx = load_library(), None
+
+    def _check(self, rc):
+        _check(self.lib, rc)
+
+
+calls = Calls()
+AT = {k: 0x1000000 * (i + 1) for i, k in enumerate(("x", "b", "h", "y", "gain", "post_gain", "dy", "dh", "dx", "db", "dgain", "dpost_gain"))}
+
+
+def norm(gradient, rows=12, **same):
+    """Validates a spec in which the operands named are at the addresses of others."""
+    names = ("b", "h", "gain", "post_gain") + (("dy", "dh", "dx", "db", "dgain", "dpost_gain") if gradient else ("x", "y"))
+    at = {n: AT[same.get(n, n)] for n in names}
+    s = calls.block_norm_spec(rows, 64, post_norm=True, **at)
+    calls._check(calls.lib.ngh_validate_block_norm(ctypes.byref(s), 1 if gradient else 0))
+
+
+def test_the_stream_and_its_gradient_may_be_updated_in_place():
+    for rows in (1, 12):
+        norm(False, rows, h="x")
+        norm(True, rows, dx="dh")
+
+
+@pytest.mark.parametrize("rows", [1, 12])
+@pytest.mark.parametrize("gradient,same", [
+    (False, dict(h="x", y="x")), (False, dict(h="x", b="x")), (False, dict(h="x", gain="x")), (False, dict(h="x", post_gain="x")), (False, dict(y="h")),
+    (True, dict(dx="dh", db="dh")), (True, dict(dx="dh", dgain="dh")), (True, dict(dx="dh", dpost_gain="dh")), (True, dict(dx="dh", post_gain="dh")),
+    (True, dict(dx="dh", gain="dh")), (True, dict(dx="dh", b="dh"))])
+def test_nothing_else_may_share_what_is_updated_in_place(gradient, same, rows):
+    with pytest.raises(HipLibraryError) as e:
+        norm(gradient, rows, **same)
+    assert e.value.code == -1 and "overlaps" in str(e.value)
