@@ -214,7 +214,7 @@ GradPlan plan_grad(const ngh_block_norm_spec* s, const Views& views, int cus) {
     g.count = __builtin_popcount((unsigned)g.vectors);
     g.spans = g.gate_whole ? 1 : rows / g.span_rows;
     g.parts_per_span = (g.span_rows + g.per_part - 1) / g.per_part;
-    g.parts = g.spans * g.parts_per_span;
+    g.parts = rows ? g.spans * g.parts_per_span : 0;                 // (no rows: the merge writes zeros)
     g.part_stride = ((size_t)s->width + 7) / 8 * 8;
     g.bytes = (size_t)g.parts * g.count * g.part_stride * 4;
     return g;
@@ -318,7 +318,7 @@ int ngh_block_norm_grad(ngh_context* ctx, const ngh_block_norm_spec* spec) {
     m.part_stride = a.part_stride;
     m.width = a.width;
     m.per_part_vectors = (unsigned)g.count;
-    m.n_parts = spec->rows ? g.parts : 0;
+    m.n_parts = g.parts;
     m.parts_per_span = g.parts_per_span;
     m.gates = g.vectors & kVecGate ? 1 : 0;
     int k = 0;

@@ -2,10 +2,12 @@
 memory, calls over nothing, counters, without a device where that is possible."""
 import ctypes
 
+import numpy as np
 import pytest
 
 from ngraph_hip.runtime import HipLibraryError, load_library, row_ops
 from ngraph_hip.runtime.hiplib import NGH_ABI_VERSION, _check
+from row_helpers import DTYPES, Pool
 
 
 class Calls(row_ops.OperatorCalls):
@@ -46,3 +48,25 @@ def test_nothing_else_may_share_what_is_updated_in_place(gradient, same, rows):
     with pytest.raises(HipLibraryError) as e:
         norm(gradient, rows, **same)
     assert e.value.code == -1 and "overlaps" in str(e.value)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")], ids="-".join)
+@pytest.mark.parametrize("width,gate_rows", [(1, 0), (64, 7), (4096, 0), (16384, 3)])
+def test_gradients_of_no_rows_are_zeros(hip_runtime, width, gate_rows, types):
+    """(an empty batch: with the workspace that the query asks for)"""
+    rt = hip_runtime
+    with Pool(rt) as pool:
+        rows = pool.rows((1, width), types[0], np.zeros((1, width)))
+        outs = {n: pool.rows((1, width), types[1]) for n in ("dgain", "dbias", "dpost_gain", "dpost_bias")}
+        untouched = {n: pool.rows((1, width), t, np.full((1, width), 3.0)) for n, t in (("dx", types[0]), ("db", types[0]), ("dgate", types[1]))}
+        gate = {"gate": rows.ptr, "dgate": untouched["dgate"].ptr, "gate_rows": gate_rows} if gate_rows else {}
+        spec = rt.block_norm_spec(0, width, "layer", DTYPES[types[0]], DTYPES[types[1]], True, h=rows.ptr, b=rows.ptr, dy=rows.ptr,
+                                  dx=untouched["dx"].ptr, db=untouched["db"].ptr, **dict({n: t.ptr for n, t in outs.items()}, **gate))
+        spec.workspace_bytes = rt.block_norm_grad_workspace(spec)
+        spec.workspace = pool.bytes(spec.workspace_bytes).ptr
+        rt.block_norm_grad(spec)
+        for n, t in outs.items():
+            assert not t.get().any(), n
+        for n, t in untouched.items():
+            assert (t.get() == 3.0).all(), n
