@@ -241,10 +241,11 @@ __global__ __launch_bounds__(kAdamBlock) void adamw_kernel(StepArgs a) {
     }
 }
 
-// The scalars of a step whose number the device counts.
+// The scalars of a step whose number the device counts (an empty plan has no place for them and only counts).
 __global__ void adamw_advance_kernel(int* step, const float* dev_lr, double lr, double beta1, double beta2, Scalars* out) {
     const int t = *step + 1;
     *step = t;
+    if (!out) return;
     if (dev_lr) lr = (double)*dev_lr;
     out->lr = (float)lr;
     out->a = (float)(lr / (1.0 - pow(beta1, (double)t)));
@@ -510,7 +511,7 @@ int ngh_adamw_step(ngh_context* ctx, ngh_adamw_plan* plan, const ngh_adamw_hyper
     if (h->dev_lr && !h->dev_step) return report(NGH_E_INVALID, "ngh_adamw_step: dev_lr without dev_step");
     DeviceScope scope(c.device);
     if (!scope.ok()) return report(NGH_E_RUNTIME, "ngh_adamw_step: the context's device cannot be made current");
-    if (plan->jobs == 0) return NGH_OK;
+    if (plan->jobs == 0 && !h->dev_step) return NGH_OK;
     StepArgs a;
     a.records = plan->dev_records;
     a.jobs = plan->dev_jobs;
@@ -528,6 +529,7 @@ int ngh_adamw_step(ngh_context* ctx, ngh_adamw_plan* plan, const ngh_adamw_hyper
         hipLaunchKernelGGL(adamw_advance_kernel, dim3(1), dim3(1), 0, c.stream, h->dev_step, h->dev_lr, h->lr, h->beta1, h->beta2,
                            plan->dev_scalars);
         NGH_HIP_TRY(hipGetLastError());
+        if (plan->jobs == 0) return NGH_OK;
         a.dev = plan->dev_scalars;
     } else {
         a.by_value.lr = (float)h->lr;

@@ -70,3 +70,23 @@ def test_gradients_of_no_rows_are_zeros(hip_runtime, width, gate_rows, types):
             assert not t.get().any(), n
         for n, t in untouched.items():
             assert (t.get() == 3.0).all(), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths", [[], [0, 0]])
+def test_an_update_of_nothing_counts(hip_runtime, lengths):
+    rt = hip_runtime
+    with Pool(rt) as pool:
+        count, lr = pool.array(np.array([4], np.int32)), pool.array(np.array([1e-3], np.float32))
+        plan = rt.adamw_plan([dict(n=n) for n in lengths])
+        for k in range(3):
+            rt.adamw_step(plan, dev_step=count.ptr, dev_lr=lr.ptr)
+            assert count.get()[0] == 5 + k
+        rt.graph_begin()
+        rt.adamw_step(plan, dev_step=count.ptr)
+        graph = rt.graph_end()
+        for k in range(2):
+            rt.graph_launch(graph)
+            assert count.get()[0] == 8 + k
+        rt.graph_free(graph)
+        rt.adamw_plan_free(plan)
