@@ -584,7 +584,11 @@ int  ngh_block_norm_grad_workspace(const ngh_block_norm_spec* spec, size_t* out_
  * fp32 scale s, the largest |m| (v) among them, and hold
  *     m: an int8  q = sign(m) rint(127 sqrt(|m| / s)),  standing for  sign(q) s (q / 127)^2
  *     v: a uint8  q = rint(255 (v / s)^(1/4)),          standing for  s (q / 255)^4
- * so that a second moment only becomes 0 where it is below 1.5e-11 of the block's largest.  The
+ * A step stores a second moment above 0 as code 1 at least; where it meets code 0 beside a first
+ * moment that is not 0 (ngh_adamw_encode rounds v below 1.5e-11 of the block's largest to 0), v counts
+ * s (0.5 / 255)^4 at least under the root, so that no step is m over eps alone.  An increase of v by
+ * less than half a step of its code is lost: where a gradient far above the others' once set a block's
+ * scale, steps of the others may reach 1.9 / sqrt(1 - beta2) times lr while it decays (fp32: about 1). The
  * update uses the moments before they are rounded.  A block in which a moment is not finite gets
  * NaN for its scale: it shows in every element of the block from the next step on.  A tensor that is
  * written may overlap nothing else of the plan.  Steps of one plan follow one another (on one stream,

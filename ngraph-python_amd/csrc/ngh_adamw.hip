@@ -13,10 +13,16 @@
 // arithmetic in this order, every operation rounded (the build contracts nothing):
 //     m: q = rint(sqrt(|m| / s) * 127), with m's sign         stands for ((q c) |q c|) s,  c = fp32(1/127)
 //     v: q = rint(sqrt(sqrt(v / s)) * 255)                    stands for ((t t) (t t)) s,  t = q fp32(1/255)
-// The roots make steps proportional to a power of the value: 1.6 % at the top of a block for both,
-// while the smallest v that is not 0 is (0.5 / 255)^4 = 1.5e-11 of the block's largest.  An element
-// whose second moment falls below that has had gradients below 4e-6 of the block's largest, so that its
-// first moment (from (0.5 / 127)^2 = 1.6e-5 of the largest on) is 0 as well: no quotient by eps alone.
+// The roots make steps proportional to a power of the value: 1.6 % at the top of a block for both, while
+// only a v below (0.5 / 255)^4 = 1.5e-11 of the block's largest rounds to 0.  After one gradient far above
+// the block's others that happens beside first moments that are not 0, for the largest m decays by beta1 a
+// step and the largest v by beta2: the step would be m over eps (gradients of 1e-5, one of 10 once: up to 765
+// times the rate, where states in fp32 take 1).  So a step stores a v above 0 as code 1 at least, and where
+// it meets code 0 beside an m that is not 0 (states encoded from fp32) it divides by the root of (0.5 / 255)^4 s
+// at least, the most that the code was rounded from: fp32's root is at most sqrt(2) times the one used.
+// What remains is the format's own: an increase of v by less than half a step of its code is lost, so that
+// v may stay at (1 - beta2) g^2 / ((1.5^4 - 1) beta2) with gradients g, at code 1, and a step reach
+// 1.9 / sqrt(1 - beta2) times the rate (8 with beta2 = 0.95, 60 with 0.999).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -81,9 +87,11 @@ __device__ __forceinline__ int first_code(float m, float s) {
     return m < 0.0f ? -q : q;
 }
 
-__device__ __forceinline__ int second_code(float v, float s) {
+// (least: the code of the smallest v above 0)
+__device__ __forceinline__ int second_code(float v, float s, int least) {
     if (!(s > 0.0f)) return 0;
-    return (int)rintf(sqrtf(sqrtf(v / s)) * 255.0f);
+    const int q = (int)rintf(sqrtf(sqrtf(v / s)) * 255.0f);
+    return v > 0.0f ? max(q, least) : q;
 }
 
 __device__ __forceinline__ float first_value(int q, float s) {
@@ -96,7 +104,9 @@ __device__ __forceinline__ float second_value(int q, float s) {
     return ((t * t) * (t * t)) * s;
 }
 
-// The codes of a lane's four moments of either kind.  They are decided by the correctly rounded quotient and
+constexpr float kLeastSecond = (float)((0.5 / 255.0) * (0.5 / 255.0) * (0.5 / 255.0) * (0.5 / 255.0));
+
+// The codes of a lane's four moments of either kind, as a step stores them.  They are decided by the correctly rounded quotient and
 // roots above, which take some 90 instructions an element for both; here approximate ones (v_rcp, v_sqrt: 1 ulp)
 // place the root within 7.5 * 2^-24 * 255 = 1.2e-4 steps of the exact chain's, so that only a root that
 // lies within 2^-12 of the border of two codes has to be worked out exactly, for the whole wavefront then (one
@@ -113,12 +123,13 @@ __device__ __forceinline__ unsigned four_codes(const float (&x)[kPer], float s) 
         const float y = SECOND ? __builtin_amdgcn_sqrtf(root) * 255.0f : copysignf(root * 127.0f, x[j]);
         const float q = rintf(y);
         close = close || !(fabsf(y - q) <= 0.5f - 0x1p-12f);
-        w |= ((unsigned)(int)q & 255u) << (8 * j);
+        const float stored = SECOND && x[j] > 0.0f ? fmaxf(q, 1.0f) : q;
+        w |= ((unsigned)(int)stored & 255u) << (8 * j);
     }
     if (__any(close)) {
         w = 0;
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) w |= ((unsigned)(SECOND ? second_code(x[j], s) : first_code(x[j], s)) & 255u) << (8 * j);
+        for (int j = 0; j < kPer; ++j) w |= ((unsigned)(SECOND ? second_code(x[j], s, 1) : first_code(x[j], s)) & 255u) << (8 * j);
     }
     return w;
 }
@@ -172,6 +183,7 @@ __global__ __launch_bounds__(kAdamBlock) void adamw_kernel(StepArgs a) {
     const float keep = 1.0f - k.lr * r.weight_decay;
     const long long first = (long long)job.chunk * (TURNS * kPiece) + threadIdx.x * kPer;
     float p[TURNS][kPer], g[TURNS][kPer], m[TURNS][kPer], v[TURNS][kPer];
+    float least[kPer] = {};                // 8 bits: what a second moment counts in the step at least
     unsigned mq[TURNS], vq[TURNS];
     float ms[TURNS], vs[TURNS];
 #pragma unroll
@@ -199,8 +211,10 @@ __global__ __launch_bounds__(kAdamBlock) void adamw_kernel(StepArgs a) {
         if constexpr (BITS == 8) {
 #pragma unroll
             for (int j = 0; j < kPer; ++j) {
-                m[t][j] = first_value((int)(signed char)(mq[t] >> (8 * j)), ms[t]);
-                v[t][j] = second_value((int)((vq[t] >> (8 * j)) & 255u), vs[t]);
+                const unsigned first = (mq[t] >> (8 * j)) & 255u, second = (vq[t] >> (8 * j)) & 255u;
+                m[t][j] = first_value((int)(signed char)first, ms[t]);
+                v[t][j] = second_value((int)second, vs[t]);
+                least[j] = second == 0 && first != 0 ? kLeastSecond * vs[t] : 0.0f;
             }
         }
         unsigned mtop = 0, vtop = 0;
@@ -211,9 +225,10 @@ __global__ __launch_bounds__(kAdamBlock) void adamw_kernel(StepArgs a) {
             v[t][j] = v[t][j] * a.beta2 + (gj * gj) * a.rest2;
             // (the step itself to a few ulp: approximate root and reciprocal, unless eps is so small that
             // what they do to the smallest numbers would show)
+            const float second = BITS == 8 && v[t][j] < least[j] ? least[j] : v[t][j];
             float step;
-            if (a.eps >= 1e-12f) step = m[t][j] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[t][j]) * k.root2 + a.eps) * k.a;
-            else step = m[t][j] / (sqrtf(v[t][j]) * k.root2 + a.eps) * k.a;
+            if (a.eps >= 1e-12f) step = m[t][j] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(second) * k.root2 + a.eps) * k.a;
+            else step = m[t][j] / (sqrtf(second) * k.root2 + a.eps) * k.a;
             p[t][j] = p[t][j] * keep - step;
             if (BITS == 8 && j < count) {
                 mtop = max(mtop, __float_as_uint(m[t][j]) & 0x7fffffffu);
@@ -285,7 +300,7 @@ __global__ __launch_bounds__(kAdamBlock) void adamw_encode_kernel(unsigned char*
         unsigned w = 0;
 #pragma unroll
         for (int j = 0; j < kPer; ++j)
-            w |= ((unsigned)(second ? second_code(v[j], s) : first_code(v[j], s)) & 255u) << (8 * j);
+            w |= ((unsigned)(second ? second_code(v[j], s, 0) : first_code(v[j], s)) & 255u) << (8 * j);
         store_codes(codes, at, count, whole, w);
         if ((threadIdx.x & 63) == 0) scales[base / NGH_ADAMW_BLOCK] = s;
     }
