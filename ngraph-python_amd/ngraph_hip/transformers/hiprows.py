@@ -64,12 +64,12 @@ def _fits(td, dtype, width_axis):
 
 
 class RowLayoutOp(og.TensorOp):
-    """x as a row kernel takes it (`_fits`); in the graph until RowLayoutPass has seen what the other passes made
-    of x."""
+    """x as a row kernel takes it (`_fits`), in other memory than the tensors `apart`, which the kernel writes; in
+    the graph until RowLayoutPass has seen what the other passes made of x."""
 
-    def __init__(self, x, width_axis, **kwargs):
+    def __init__(self, x, width_axis, apart=(), **kwargs):
         super(RowLayoutOp, self).__init__(args=(x,), axes=x.axes, dtype=x.dtype, **kwargs)
-        self.width_axis = width_axis
+        self.width_axis, self.apart = width_axis, apart
         self.deriv_handler = _Adjoint(lambda add_delta, adjoints, delta: add_delta(adjoints, self.args[0], delta))
 
 
@@ -80,7 +80,7 @@ class RowLayoutPass(PeepholeGraphPass):
         if isinstance(op, RowLayoutOp):
             x, = args
             td = _td(x)
-            if _fits(td, op.dtype, op.width_axis):
+            if _fits(td, op.dtype, op.width_axis) and not any(t.tensor_description().base == td.base for t in op.apart):
                 self.replace_op(op, x)
             elif td.dtype == op.dtype:
                 self.replace_op(op, og.ContiguousOp(x))
@@ -326,7 +326,8 @@ class AdamWOp(og.Op):
             if not g.axes.is_equal_set(v.axes):
                 raise ValueError("AdamW: a gradient with axes {} for a variable with {}".format(g.axes, v.axes))
             _check_dtype(g, (F32, F16), "AdamW: gradient")
-            args.append(_dense(og.axes_with_order(g, v.axes)))
+            # (the gradient of sum(v * w) in v is w itself)
+            args.append(RowLayoutOp(og.axes_with_order(g, v.axes), None, apart=variables))
         for what, kinds in (("variables", set(v.dtype for v in variables)), ("gradients", set(a.dtype for a in args))):
             if len(kinds) > 1:
                 raise ValueError("AdamW: %s of several dtypes; use an op for each" % what)

@@ -257,6 +257,53 @@ def test_flex_operands_behind_a_view_are_refused():
         t.close()
 
 
+def product_of_variables(state_bits):
+    """sum(v * w * 1) + sum(v * u): the gradient of either factor is the other one's memory."""
+    F, = axes("F")
+    rs = np.random.RandomState(7)
+    values = [rs.normal(0, 1, 20).astype(f32) for _ in range(3)]
+    v, w, u = variables = [ng.variable([F], initial_value=a) for a in values]
+    opt = neon.AdamW(learning_rate=0.25, weight_decay=0.0, state_bits=state_bits)
+    step = opt.minimize(ng.sum(v * w, out_axes=()) + ng.sum(v * u, out_axes=()), variables=variables)
+    return variables, values, opt, step
+
+
+@pytest.mark.parametrize("state_bits", [32, 8])
+def test_a_gradient_that_is_another_variable_is_copied(state_bits):
+    variables, values, opt, step = product_of_variables(state_bits)
+    t, kernels = lowered(step)
+    try:
+        update, = [k for k in kernels if isinstance(k, hiprows.AdamWKernel)]
+        held = [x.tensor_description().base for x in variables]
+        for a in update.op.args:
+            assert_rows_in_order(_td(a.forwarded), np.dtype(f32))
+            assert _td(a.forwarded).base not in held
+    finally:
+        t.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("state_bits", [32, 8])
+def test_updates_by_gradients_that_are_other_variables(hip_runtime, state_bits):
+    """Steps of 0.25 by the signs of the values before the step, first moments a tenth of them (8 bits: to half a code)."""
+    variables, values, opt, step = product_of_variables(state_bits)
+    t = ngt.make_transformer_factory("hipgpu")()
+    try:
+        f, read = t.computation([step]), [t.computation(x) for x in variables]
+        f()
+        after = [np.array(r()) for r in read]
+        m = [np.array(t.get_tensor_view_value(x)) for x in opt.update.m]
+    finally:
+        t.close()
+    v, w, u = [a.astype(f64) for a in values]
+    for a, before, g, mk in zip(after, (v, w, u), (w + u, v, v), m):
+        np.testing.assert_allclose(a, before - 0.25 * g / (np.abs(g) + 1e-8), rtol=0, atol=2.0 ** -24 * (12 * 0.25 + 4 * np.abs(before).max()))
+        if state_bits == 32:
+            np.testing.assert_allclose(mk, (1 - 0.9) * g, rtol=6 * 2.0 ** -24, atol=0)
+        else:
+            np.testing.assert_allclose(mk, np.sign(g) * 127 * np.sqrt(np.abs(g) / np.abs(g).max()), rtol=0, atol=0.501)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("name", sorted(CASES))
 def test_results_against_float64(hip_runtime, name):
