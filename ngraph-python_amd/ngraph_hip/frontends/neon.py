@@ -264,8 +264,9 @@ class AdamW(Optimizer):
     The reference's Adam (frontends/neon/optimizer.py:446-470, `Adam` above) is a kernel for each
     variable, keeps epsilon outside the bias correction and decays nothing.  learning_rate may be a scalar
     op.  `decayed` chooses the variables that decay (default: those of two axes or more, which leaves
-    gains and biases out).  `minimize` returns an op whose AdamWOp is kept as `update`: its `step`, `m`
-    and `v` are persistent tensors."""
+    gains and biases out).  `minimize` returns an op whose AdamWOps, one for every pair of dtypes of variables and
+    gradients, are kept as `updates` (the first as `update`): `step`, `m` and `v` of each are persistent
+    tensors."""
 
     def __init__(self, learning_rate=1e-3, beta_1=0.9, beta_2=0.999, epsilon=1e-8, weight_decay=0.01, state_bits=32, decayed=None,
                  **clipping):
@@ -273,10 +274,10 @@ class AdamW(Optimizer):
         self.lrate, self.beta_1, self.beta_2, self.epsilon = learning_rate, beta_1, beta_2, epsilon
         self.weight_decay, self.state_bits = weight_decay, state_bits
         self.decayed = decayed if decayed is not None else lambda variable: len(variable.axes) >= 2
-        self.update = None
+        self.updates, self.update = [], None
 
     def minimize(self, cost_func, variables=None):
-        from ngraph_hip.transformers.hiprows import AdamWOp
+        from ngraph_hip.transformers.hiprows import AdamWOp, RowLayoutOp
         batch_cost = ng.sum(cost_func, out_axes=())
         batch_axis = cost_func.axes.batch_axis()
         share = 1.0 if batch_axis is None else 1.0 / batch_axis.length
@@ -290,9 +291,23 @@ class AdamW(Optimizer):
             # (the values that are clipped are those of the mean gradient)
             grads = [clip_gradient_value(g * share, self.gradient_clip_value) for g in grads]
             share = 1.0
-        self.update = AdamWOp(variables, grads, self.lrate, self.beta_1, self.beta_2, self.epsilon,
-                              [self.weight_decay if self.decayed(v) else 0.0 for v in variables], self.state_bits, share, factor)
-        steps = [self.update]
+        grads = [ng.axes_with_order(g, v.axes) for v, g in zip(variables, grads)]
+        kinds = []
+        for v, g in zip(variables, grads):
+            if (v.dtype, g.dtype) not in kinds:
+                kinds.append((v.dtype, g.dtype))
+        steps = []
+        if len(kinds) > 1:
+            # (every gradient is taken, and copied where it is a variable, before the first of the updates)
+            grads = [RowLayoutOp(g, None, apart=variables) for g in grads]
+            steps.append(ng.doall(grads))
+        self.updates = []
+        for kind in kinds or [None]:
+            chosen = [(v, g) for v, g in zip(variables, grads) if (v.dtype, g.dtype) == kind]
+            self.updates.append(AdamWOp([v for v, _ in chosen], [g for _, g in chosen], self.lrate, self.beta_1, self.beta_2, self.epsilon,
+                                        [self.weight_decay if self.decayed(v) else 0.0 for v, _ in chosen], self.state_bits, share, factor))
+        self.update = self.updates[0]
+        steps += self.updates
         if self.weight_clip_value is not None:
             steps += [ng.assign(v, clip_weight_value(v, self.weight_clip_value)) for v in variables]
         return ng.sequential(steps + [batch_cost])

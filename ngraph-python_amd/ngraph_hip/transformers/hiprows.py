@@ -330,7 +330,7 @@ class AdamWOp(og.Op):
             args.append(RowLayoutOp(og.axes_with_order(g, v.axes), None, apart=variables))
         for what, kinds in (("variables", set(v.dtype for v in variables)), ("gradients", set(a.dtype for a in args))):
             if len(kinds) > 1:
-                raise ValueError("AdamW: %s of several dtypes; use an op for each" % what)
+                raise ValueError("AdamW: %s of several dtypes; use an op for each (neon's AdamW does)" % what)
         self.variables, self.n = list(variables), len(variables)
         self.grad_dtype = args[0].dtype if args else F32
         self.beta_1, self.beta_2, self.epsilon = float(beta_1), float(beta_2), float(epsilon)
