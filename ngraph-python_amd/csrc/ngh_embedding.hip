@@ -18,7 +18,7 @@
 //      rows lie in one unit is finished there; parts of a token that crosses units go to the
 //      workspace, so that one frequent token is spread over as many wavefronts as many rare ones.
 //      In the same launch other workgroups clear the rows whose token the sorted list does not hold; the
-//      launches of the sort, which leave the memory idle, have cleared the table's first rows altogether.
+//      launches that rank chunks, which leave the memory idle, have cleared the table's first rows altogether.
 //   3. merge.  A workgroup for each unit in which a crossing token begins adds its parts in order.
 // Measured: 1999 places into [20011, 301] fp32 12.4 us (latency, and 24 MB to clear); 16384 bf16 rows into [65536, 1024]
 // fp32 78 us (sort 33 with half of the table cleared beside it, sums and the other half 39, merge 5.5); 131072 rows
@@ -120,13 +120,13 @@ struct SortArgs {
                                  // before, and a row of all tiles'
     unsigned tiles, scanned;
     int shift, bits;
-    // workgroups behind the first `workers` clear [clear, clear + clear_bytes), from a 16-byte boundary
+    // ranking launches: workgroups behind the first `workers` clear [clear, clear + clear_bytes), from a 16-byte boundary
     unsigned workers;
     char* clear;
     unsigned long long clear_bytes;
 };
 
-// Workgroups of a launch of the sort that do not sort: each clears its share of a part of the table.
+// Workgroups of a launch that ranks chunks which do not sort: each clears its share of a part of the table.
 __device__ __forceinline__ bool clears(const SortArgs& a) {
     if (blockIdx.x < a.workers) return false;
     const uint4 zero = make_uint4(0, 0, 0, 0);
@@ -269,7 +269,6 @@ __device__ __forceinline__ unsigned tile_key(const SortArgs& a, unsigned i) {
 template <bool FIRST>
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a) {
     __shared__ unsigned hist[kTileDigits];
-    if (clears(a)) return;
     for (unsigned i = threadIdx.x; i < kTileDigits; i += kSortThreads) hist[i] = 0;
     __syncthreads();
 #pragma unroll
@@ -324,7 +323,6 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortArgs a) 
     __shared__ unsigned start[kTileDigits];
     __shared__ unsigned part[kTileDigits];
     __shared__ unsigned sh[kSortWaves];
-    if (clears(a)) return;
     const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const unsigned digits = 1u << a.bits;
     unsigned key[kTileItems], place[kTileItems], rank[kTileItems];
