@@ -257,7 +257,8 @@ class Adam(Optimizer):
 
 
 class AdamW(Optimizer):
-    """Adam with decoupled weight decay, every variable updated in one launch, moments in fp32 or 8 bits:
+    """Adam with decoupled weight decay, all variables of a dtype updated in one launch (behind one of a single lane that
+    counts the steps), moments in fp32 or 8 bits:
 
         p = p (1 - lr weight_decay) - lr / (1 - beta_1^t) m / (sqrt(v) / sqrt(1 - beta_2^t) + epsilon)
 
